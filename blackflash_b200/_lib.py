@@ -31,6 +31,11 @@ EXPORTED = (
     "blackflash_ring_forward",
     "blackflash_ring_status",
     "blackflash_ring_destroy",
+    "blackflash_window_fwd",
+    "blackflash_decode_workspace_bytes",
+    "blackflash_window_decode",
+    "blackflash_prefix_decode",
+    "blackflash_rotary",
     "blackflash_fwd_timeout_probe",
     "blackflash_fwd_debug_s",
     "blackflash_fwd_trace",
@@ -41,7 +46,19 @@ EXPORTED = (
 _lock = threading.Lock()
 _lib = None
 
+# Element types (BF_DTYPE_*).
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+
+
+class View(ctypes.Structure):
+    """bf_view: address and the element strides of batch, head and token."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_longlong * 3)]
+
+
+
 _vp, _fp, _i, _ll, _f = ctypes.c_void_p, ctypes.POINTER(ctypes.c_float), ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+
+_view = ctypes.POINTER(View)
 
 _SIGS = {
     "blackflash_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp]),
@@ -63,6 +80,11 @@ _SIGS = {
     "blackflash_fwd_timeout_probe": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, ctypes.c_ulonglong, _vp]),
     "blackflash_fwd_debug_s": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp]),
     "blackflash_fwd_trace": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
+    "blackflash_window_fwd": (_i, [_view] * 3 + [_vp, _vp] + [_i] * 8 + [_f, _i, _vp]),
+    "blackflash_decode_workspace_bytes": (_ll, [_i] * 9),
+    "blackflash_window_decode": (_i, [_vp, _view, _view, _vp, _vp, _vp, _vp, _ll] + [_i] * 8 + [_f, _i, _vp]),
+    "blackflash_prefix_decode": (_i, [_vp] + [_view] * 4 + [_vp, _vp, _vp, _vp, _ll] + [_i] * 7 + [_f, _i, _vp]),
+    "blackflash_rotary": (_i, [_view, _view, _vp, _vp, _vp, _i, _i, _vp] + [_i] * 7 + [_f, _i, _i, _vp]),
     "blackflash_last_error": (ctypes.c_char_p, []),
     "blackflash_abi_version": (_i, []),
 }

@@ -21,8 +21,10 @@ HARNESS_PATH = os.path.join(LIB_DIR, "flash_attn")
 # `import blackflash_cuda` resolves as it does for the reference's installed extension.
 EXT_SRC = os.path.join(CSRC, "torch_ext.cpp")
 
-SOURCES = ["fa_fwd_sm100.cu", "capi.cu", "lse_merge.cu", "noalloc.cu", "ring_ipc.cu"]
-HEADERS = ["sm100_ptx.cuh", "fa_fwd_sm100.h", "fa_fwd_sm100_d128.cuh", "fa_bwd_sm100.cuh"]
+SOURCES = ["fa_fwd_sm100.cu", "capi.cu", "lse_merge.cu", "noalloc.cu", "ring_ipc.cu", "window_sm100.cu", "decode.cu",
+           "rotary.cu"]
+HEADERS = ["sm100_ptx.cuh", "fa_fwd_sm100.h", "fa_fwd_sm100_d128.cuh", "fa_bwd_sm100.cuh", "launch_sm100.h", "views.h",
+           "window_fwd_sm100.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", os.path.join(REPO_DIR, "include")]
 
@@ -58,7 +60,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     deps += [os.path.join(REPO_DIR, "include", f) for f in ("blackflash_b200.h", "blackflash_b200_diag.h", "flash_attn.cuh")]
     if force or _stale(LIB_PATH, deps):
         tmp = LIB_PATH + ".tmp"
-        cmd = [_nvcc(), *ARCH, *COMMON, "-shared", "-o", tmp, *[os.path.join(CSRC, f) for f in SOURCES]]
+        cmd = [_nvcc(), *ARCH, *COMMON, "--threads", "0", "-shared", "-o", tmp, *[os.path.join(CSRC, f) for f in SOURCES]]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         _run(cmd, verbose)

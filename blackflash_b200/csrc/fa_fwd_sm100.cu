@@ -40,6 +40,7 @@
 // word and the kernel unwinds instead of spinning forever.
 #include "sm100_ptx.cuh"
 #include "fa_fwd_sm100.h"
+#include "launch_sm100.h"
 
 #include <cuda_bf16.h>
 #include <math.h>
@@ -682,22 +683,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ============================================================================ host side
 namespace {
 
-typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-PFN_encodeTiled get_encode_fn() {
-    static PFN_encodeTiled fn = nullptr;
-    if (!fn) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-            qres == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_encodeTiled>(ptr);
-    }
-    return fn;
-}
-
 // [BH][rows][64] bf16 viewed as a 3-D tensor; 64 x 128-row boxes with 128-byte
 // swizzle. Rows past `rows` inside a slice load as zero and are never stored.
 // For d = 128 the same 64-column box is loaded twice per tile (columns 0 and 64).
@@ -761,30 +746,6 @@ int cached_map(CUtensorMap* m, const void* base, long long bh, int rows, int d =
     g_map_cache_next = (g_map_cache_next + 1) % kMapCacheSize;
     if (g_map_cache_used < kMapCacheSize) ++g_map_cache_used;
     return BF_OK;
-}
-
-// Launch with programmatic stream serialisation: the kernel's set-up overlaps the tail
-// of the previous kernel on the stream (the kernels wait with griddepcontrol.wait
-// before touching global memory).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
-                       Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    // BLACKFLASH_NO_PDL=1 launches with plain stream order (read once per process).
-    static const bool no_pdl = [] {
-        const char* v = getenv("BLACKFLASH_NO_PDL");
-        return v && v[0] && v[0] != '0';
-    }();
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = no_pdl ? 0 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 template <bool kF32Out>
@@ -1041,7 +1002,7 @@ int bf_bwd_launch(const BfBwdArgs* a) {
 }
 
 extern "C" int blackflash_status(int reset, unsigned* out) {
-    unsigned v = 0;
+    unsigned v = 0, w = 0;
     cudaError_t e = cudaMemcpyFromSymbol(&v, bfk::g_wait_status, sizeof(v));
     if (e != cudaSuccess) return bf_set_error(BF_ERR_CUDA, cudaGetErrorString(e));
     if (reset) {
@@ -1049,6 +1010,8 @@ extern "C" int blackflash_status(int reset, unsigned* out) {
         e = cudaMemcpyToSymbol(bfk::g_wait_status, &zero, sizeof(zero));
         if (e != cudaSuccess) return bf_set_error(BF_ERR_CUDA, cudaGetErrorString(e));
     }
-    if (out) *out = v;
+    const int rc = bf_window_wait_status(reset, &w);  // the windowed kernels' own word
+    if (rc != BF_OK) return rc;
+    if (out) *out = v ? v : w;
     return BF_OK;
 }

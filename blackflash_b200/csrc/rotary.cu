@@ -1,0 +1,234 @@
+// Rotary positions: pair i of a token at position n is turned by the angle n * freq[i] and
+// stretched by an amplitude,
+//   (u, w) -> a (u cos - w sin, u sin + w cos),
+// for Q and K in one launch. Pairs are neighbours (interleaved) or the two halves of the
+// rotated part; the columns past it are copied. The gradient is the same map with the
+// angle's sign turned.
+//
+// Bound by memory: every element is read once and written once. The angle needs 64 bits,
+// because at position 10^6 a 32-bit product is off by 0.06 rad: it is formed in turns
+// (freq / 2 pi, in fp64), reduced to [-1/2, 1/2] there, and only then taken to fp32 and
+// sincospi. A block does this once for its tokens and all of their heads, into shared
+// memory, so the fp64 work is one product and one rounding per (token, pair).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+#include <string.h>
+
+#include "sm100_ptx.cuh"
+#include "views.h"
+
+namespace bfk {
+namespace rot {
+
+struct Params {
+    const char* x[2];       // Q, K (null: absent)
+    char* y[2];             // contiguous [B, H, N, d]
+    long long xs[2][3];     // byte strides of batch, head, token
+    int heads[2];
+    const void* positions;  // [N] or [B, N], int32 or int64
+    long long pos_stride;   // 0 or N
+    const double* freqs;    // [rot / 2], radians per position
+    float amplitude, sign;
+    long long tokens;       // B * N
+    int n, d, rot, pos64;
+    int tile;               // tokens of a block
+    int head_split;         // blocks along the heads
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T, int V>
+struct __align__(sizeof(T) * V) Vec {
+    T e[V];
+};
+
+constexpr int kBlock = 256;
+constexpr int kMaxPairs = 512;  // (token, pair) entries of a block's table
+
+// A work item is V consecutive columns of one row: of the first half with their partners of
+// the second half (half layout), of the rotated part (interleaved), or copied columns.
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kBlock) rotary_kernel(const Params p) {
+    __shared__ float2 cs[kMaxPairs];
+    const int half = p.rot / 2;
+    const long long t0 = (long long)blockIdx.x * p.tile;
+    const int nt = (int)min((long long)p.tile, p.tokens - t0);
+    griddep_launch_dependents();
+    griddep_wait();
+    for (int i = threadIdx.x; i < nt * half; i += kBlock) {
+        const int t = i / half, pr = i - t * half;
+        const long long tok = t0 + t;
+        const long long b = tok / p.n, at = b * p.pos_stride + (tok - b * p.n);
+        const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
+                                      : (long long)reinterpret_cast<const int*>(p.positions)[at];
+        const double turns = (double)pos * (p.freqs[pr] * 0.15915494309189533577);
+        const double angle = 2.0 * (turns - rint(turns));  // in units of pi, [-1, 1]
+        const float hi = (float)angle;
+        float s, c;
+        sincospif(hi, &s, &c);
+        // First-order step for what the cast to fp32 dropped (up to 2^-24 of the angle).
+        const float lo = (float)(angle - (double)hi) * 3.14159265f;
+        cs[i] = make_float2((c - s * lo) * p.amplitude, (s + c * lo) * p.amplitude * p.sign);
+    }
+    __syncthreads();
+
+    // Items of a row: the rotated ones, then the copied ones.
+    const int rot_items = kInterleaved ? p.rot / V : half / V;
+    const int row_items = rot_items + (p.d - p.rot) / V;
+    const int all_heads = p.heads[0] + p.heads[1];
+    const int h0 = (int)((long long)all_heads * blockIdx.y / p.head_split);
+    const int h1 = (int)((long long)all_heads * (blockIdx.y + 1) / p.head_split);
+    const int per_token = (h1 - h0) * row_items;
+    using VT = Vec<T, V>;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < nt * per_token; i += kBlock) {
+        const int t = i / per_token;
+        const int rest = i - t * per_token;
+        const int hh = h0 + rest / row_items, item = rest % row_items;
+        const int which = hh >= p.heads[0];
+        const int h = which ? hh - p.heads[0] : hh;
+        const long long tok = t0 + t;
+        const long long b = tok / p.n, n = tok - b * p.n;
+        const T* x = reinterpret_cast<const T*>(p.x[which] + b * p.xs[which][0] + h * p.xs[which][1] + n * p.xs[which][2]);
+        T* y = reinterpret_cast<T*>(p.y[which]) + ((b * p.heads[which] + h) * p.n + n) * p.d;
+        const float2* tab = cs + t * half;
+        if (item >= rot_items) {
+            const int c = p.rot + (item - rot_items) * V;
+            *reinterpret_cast<VT*>(y + c) = *reinterpret_cast<const VT*>(x + c);
+        } else if constexpr (kInterleaved) {
+            const int c = item * V;
+            const VT a = *reinterpret_cast<const VT*>(x + c);
+            VT r;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 w = tab[(c + e) >> 1];
+                const float u = to_f<T>(a.e[e]), v = to_f<T>(a.e[e + 1]);
+                r.e[e] = from_f<T>(u * w.x - v * w.y);
+                r.e[e + 1] = from_f<T>(u * w.y + v * w.x);
+            }
+            *reinterpret_cast<VT*>(y + c) = r;
+        } else {
+            const int c = item * V;
+            const VT a = *reinterpret_cast<const VT*>(x + c), bq = *reinterpret_cast<const VT*>(x + half + c);
+            VT r, q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float2 w = tab[c + e];
+                const float u = to_f<T>(a.e[e]), v = to_f<T>(bq.e[e]);
+                r.e[e] = from_f<T>(u * w.x - v * w.y);
+                q.e[e] = from_f<T>(u * w.y + v * w.x);
+            }
+            *reinterpret_cast<VT*>(y + c) = r;
+            *reinterpret_cast<VT*>(y + half + c) = q;
+        }
+    }
+}
+
+template <typename T, int V, bool kInterleaved>
+int launch(const Params& p, dim3 grid, cudaStream_t stream) {
+    return launch_error(launch_pdl(rotary_kernel<T, V, kInterleaved>, grid, kBlock, 0, stream, p));
+}
+
+// V = 16 bytes where every piece of a row is whole 16-byte vectors, else the largest power
+// of two that divides the pieces (a pair for the interleaved layout, one column for halves).
+template <typename T>
+int launch_v(const Params& p, int v, bool interleaved, dim3 grid, cudaStream_t stream) {
+    constexpr int kMax = 16 / (int)sizeof(T);
+    if (interleaved) {
+        if (v == kMax) return launch<T, kMax, true>(p, grid, stream);
+        return launch<T, 2, true>(p, grid, stream);
+    }
+    if (v == kMax) return launch<T, kMax, false>(p, grid, stream);
+    return launch<T, 1, false>(p, grid, stream);
+}
+
+}  // namespace rot
+}  // namespace bfk
+
+extern "C" int blackflash_rotary(const bf_view* Q, const bf_view* K, void* Q_out, void* K_out, const void* positions,
+                                 int positions_64, int positions_per_batch, const double* freqs, int B, int Hq, int Hk,
+                                 int N, int d, int rotary_dim, int interleaved, float amplitude, int inverse, int dtype,
+                                 void* stream) {
+    bf_set_error(BF_OK, "");
+    if (B <= 0 || N <= 0 || Hq < 0 || Hk < 0 || Hq + Hk <= 0)
+        return bf_set_error(BF_ERR_ARG, "empty problem: B, N and the heads must be >= 1");
+    if (Hq > 65536 || Hk > 65536) return bf_set_error(BF_ERR_ARG, "more than 65536 heads");
+    if (d <= 0 || d > 1024 || d % 2 || rotary_dim < 2 || rotary_dim > d || rotary_dim % 2)
+        return bf_set_error(BF_ERR_ARG, "need an even d <= 1024 and an even rotary_dim in [2, d]");
+    if (!positions || !freqs) return bf_set_error(BF_ERR_ARG, "null pointer");
+    if (!isfinite(amplitude)) return bf_set_error(BF_ERR_ARG, "amplitude must be finite");
+    if (dtype != BF_DTYPE_BF16 && dtype != BF_DTYPE_F16 && dtype != BF_DTYPE_F32)
+        return bf_set_error(BF_ERR_ARG, "dtype must be bf16, fp16 or fp32");
+    const int size = dtype == BF_DTYPE_F32 ? 4 : 2;
+    bfk::rot::Params p;
+    memset(&p, 0, sizeof(p));
+    const bf_view* in[2] = {Q, K};
+    void* out[2] = {Q_out, K_out};
+    const int heads[2] = {Hq, Hk};
+    const int full = 16 / size;
+    // Every boundary inside a row, and every row's start, on whole vectors?
+    bool vec = d % full == 0 && rotary_dim % full == 0 && (interleaved || rotary_dim / 2 % full == 0);
+    for (int i = 0; i < 2; ++i) {
+        p.heads[i] = heads[i];
+        if (!heads[i]) continue;
+        if (!in[i] || !in[i]->data || !out[i]) return bf_set_error(BF_ERR_ARG, "null pointer");
+        const uintptr_t at = reinterpret_cast<uintptr_t>(in[i]->data), to = reinterpret_cast<uintptr_t>(out[i]);
+        if (at % (2 * size) || to % (2 * size)) return bf_set_error(BF_ERR_ARG, "Q and K must start on whole pairs");
+        vec = vec && at % 16 == 0 && to % 16 == 0;
+        p.x[i] = reinterpret_cast<const char*>(in[i]->data);
+        p.y[i] = reinterpret_cast<char*>(out[i]);
+        const int n[3] = {B, heads[i], N};
+        for (int k = 0; k < 3; ++k) {
+            const long long s = n[k] > 1 ? in[i]->stride[k] : 0;
+            if (s < 0 || s % 2) return bf_set_error(BF_ERR_ARG, "strides must be even and not negative");
+            vec = vec && s % full == 0;
+            p.xs[i][k] = s * size;
+        }
+    }
+    const int v = vec ? full : (interleaved ? 2 : 1);
+    p.positions = positions;
+    p.pos64 = positions_64 != 0;
+    p.pos_stride = positions_per_batch ? N : 0;
+    p.freqs = freqs;
+    p.amplitude = amplitude;
+    p.sign = inverse ? -1.f : 1.f;
+    p.tokens = (long long)B * N;
+    p.n = N;
+    p.d = d;
+    p.rot = rotary_dim;
+    // Tokens of a block: enough that one pass of its threads fills the table, fewer where that
+    // would leave multiprocessors without a block; then the heads are split too.
+    int tile = bfk::rot::kBlock / (rotary_dim / 2);
+    if (tile < 1) tile = 1;
+    if (tile > 8) tile = 8;
+    const long long even = (p.tokens + 2 * kPlanSms - 1) / (2 * kPlanSms);
+    if (even < tile) tile = (int)even;
+    p.tile = tile;
+    const long long blocks = (p.tokens + tile - 1) / tile;
+    if (blocks > 0x7fffffffLL) return bf_set_error(BF_ERR_ARG, "problem too large for one launch");
+    long long hs = (2 * kPlanSms + blocks - 1) / blocks;
+    if (hs > Hq + Hk) hs = Hq + Hk;
+    if (hs > 65535) hs = 65535;
+    p.head_split = (int)hs;
+    const dim3 grid((unsigned)blocks, (unsigned)hs);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (dtype == BF_DTYPE_F32) return bfk::rot::launch_v<float>(p, v, interleaved != 0, grid, st);
+    if (dtype == BF_DTYPE_F16) return bfk::rot::launch_v<__half>(p, v, interleaved != 0, grid, st);
+    return bfk::rot::launch_v<__nv_bfloat16>(p, v, interleaved != 0, grid, st);
+}

@@ -150,6 +150,78 @@ int blackflash_ring_forward(void* ring, const void* Q, const void* K, const void
 int blackflash_ring_status(void* ring, int reset, unsigned* out);
 int blackflash_ring_destroy(void* ring);
 
+/* Element types of the entry points below. */
+#define BF_DTYPE_BF16 0
+#define BF_DTYPE_F16 1
+#define BF_DTYPE_F32 2
+
+/*
+ * A [batch, heads, tokens, d] tensor whose last axis is contiguous: its address and the
+ * strides of the first three axes, in elements. Unless an entry point says otherwise the
+ * address is 16-byte aligned and the strides are positive multiples of 16 bytes (the stride
+ * of an axis with one element is not looked at).
+ */
+typedef struct {
+    const void* data;
+    long long stride[3];
+} bf_view;
+
+/*
+ * Causal attention with a sliding window and sinks, grouped KV heads. No counterpart in the
+ * reference.
+ *   Q: [B, Hq, Nq, d], K, V: [B, Hkv, Nkv, d], bf16 or fp16, d = 64 or 128, Hq a multiple
+ *   of Hkv; query head h reads KV head h / (Hq / Hkv). O: [B, Hq, Nq, d] contiguous.
+ *   lse: [B, Hq, Nq] fp32 natural logsumexp, optional.
+ * Query i stands at position p = i + Nkv - Nq (the last query at the last key) and sees the
+ * keys j <= p with j > p - window or j < sinks. window >= Nkv is plain causal attention. A
+ * query that sees no key (p < 0) gets O = 0 and lse = -inf. scale must be positive.
+ * K and V must be finite in every row: a masked key has weight 0, but it takes part in the
+ * matrix products of its 128-row tile, and 0 times an infinity or NaN is NaN.
+ */
+int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const bf_view* V, void* O, float* lse, int B, int Hq,
+                          int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale, int dtype, void* stream);
+
+/*
+ * Decoding steps: T >= 1 new tokens of each sequence against its cache. No counterpart in
+ * the reference.
+ *   Q: [B, Hq, T, d] contiguous; K, V: caches [B, Hkv, C, d] of any strides; lengths: [B]
+ *   int32 on the device, the tokens of each cache in use, the T new ones among them (held
+ *   to 0 .. C). O: [B, Hq, T, d] contiguous; lse: [B, Hq, T] fp32, optional.
+ * New token t of sequence b stands at position p = lengths[b] - T + t. In
+ * blackflash_window_decode it sees the keys j <= p with j > p - window or j < sinks; in
+ * blackflash_prefix_decode all P keys of the prefix Kp, Vp [Hkv, P, d] that the sequences
+ * share (axis 0 of their views is not looked at; its one batch element serves all) and
+ * the keys j <= p of its own cache. P or C may be 0 (then the matching views may be null).
+ * A token that sees no key gets O = 0 and lse = -inf. Cache rows at lengths[b] and after are
+ * never read.
+ *   workspace: device memory of blackflash_decode_workspace_bytes(...) bytes (P = 0 for
+ *   blackflash_window_decode; window = INT_MAX and sinks = 0 for blackflash_prefix_decode),
+ *   16-byte aligned, overwritten; null where that is 0. It returns -1 for bad sizes. Calls
+ *   that overlap on the GPU need workspaces of their own.
+ */
+long long blackflash_decode_workspace_bytes(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, int sinks);
+int blackflash_window_decode(const void* Q, const bf_view* K, const bf_view* V, const int* lengths, void* O, float* lse,
+                             void* workspace, long long workspace_bytes, int B, int Hq, int Hkv, int T, int C, int d,
+                             int window, int sinks, float scale, int dtype, void* stream);
+int blackflash_prefix_decode(const void* Q, const bf_view* Kp, const bf_view* Vp, const bf_view* K, const bf_view* V,
+                             const int* lengths, void* O, float* lse, void* workspace, long long workspace_bytes, int B,
+                             int Hq, int Hkv, int T, int P, int C, int d, float scale, int dtype, void* stream);
+
+/*
+ * Rotary positions of Q [B, Hq, N, d] and K [B, Hk, N, d] (bf16, fp16 or fp32; one of Hq, Hk
+ * may be 0), into contiguous Q_out, K_out of the same type, which may not overlap the inputs.
+ * Pair i of a token at position n is turned by n * freqs[i] radians and multiplied by
+ * amplitude; with interleaved != 0 pair i is the columns (2i, 2i + 1), else
+ * (i, i + rotary_dim / 2). Columns from rotary_dim on are copied. inverse != 0 turns the
+ * other way, which is the gradient's map.
+ *   positions: [N], or [B, N] with positions_per_batch != 0; int32, or int64 with
+ *   positions_64 != 0. freqs: [rotary_dim / 2] fp64. Both on the device.
+ *   d even and at most 1024; addresses whole pairs, strides even and >= 0 (0 broadcasts).
+ */
+int blackflash_rotary(const bf_view* Q, const bf_view* K, void* Q_out, void* K_out, const void* positions,
+                      int positions_64, int positions_per_batch, const double* freqs, int B, int Hq, int Hk, int N, int d,
+                      int rotary_dim, int interleaved, float amplitude, int inverse, int dtype, void* stream);
+
 /*
  * Wait-timeout status of the current device. It is synchronous: it reads a
  * device word that a kernel sets when one of its bounded mbarrier waits gives

@@ -1,0 +1,125 @@
+"""Position-aware operators on the CPU: argument checks of the C ABI and of the Python
+layer, workspace plans, frequency tables."""
+import math
+
+import pytest
+import torch
+
+
+def view(lib, data=16, strides=(64, 64, 64)):
+    import ctypes
+
+    from blackflash_b200 import _lib
+    return _lib.View(data, (ctypes.c_longlong * 3)(*strides))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from blackflash_b200 import _lib
+    from blackflash_b200.build import build_lib
+    build_lib()
+    return _lib.load()
+
+
+WINDOW = dict(B=1, Hq=2, Hkv=1, Nq=8, Nkv=8, d=64, window=4, sinks=0, scale=0.125, dtype=0)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(B=0), b"empty"), (dict(Nkv=0), b"empty"), (dict(Hq=3, Hkv=2), b"multiple"), (dict(d=96), b"d=64"),
+    (dict(window=0), b"window"), (dict(sinks=-1), b"sinks"), (dict(scale=0.0), b"scale"),
+    (dict(scale=math.nan), b"scale"), (dict(scale=-1.0), b"scale"), (dict(dtype=2), b"dtype"),
+    (dict(Nq=(1 << 30) + 1), b"2^30"), (dict(B=70000, Hq=40000, Hkv=40000), b"too large"),
+])
+def test_window_fwd_refuses_sizes(lib, change, text):
+    a = {**WINDOW, **change}
+    v = view(lib, strides=(1 << 20, 1 << 14, 64))
+    rc = lib.blackflash_window_fwd(v, v, v, 16, None, *(a[x] for x in WINDOW), None)
+    assert rc == 1 and text in lib.blackflash_last_error(), lib.blackflash_last_error()
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(data=0), b"null"), (dict(data=24), b"aligned"), (dict(strides=(64, 64, 60)), b"strides"),
+    (dict(strides=(64, 0, 64)), b"strides"), (dict(strides=(64, 64, -64)), b"strides"),
+])
+def test_views_are_checked(lib, bad, text):
+    ok = view(lib)
+    for i in range(3):
+        views = [ok, ok, ok]
+        views[i] = view(lib, **bad)
+        rc = lib.blackflash_window_fwd(*views, 16, None, *{**WINDOW, "Hkv": 2}.values(), None)
+        assert rc == 1 and text in lib.blackflash_last_error()
+    rc = lib.blackflash_window_fwd(ok, ok, ok, 8, None, *WINDOW.values(), None)
+    assert rc == 1 and b"O must" in lib.blackflash_last_error()
+
+
+def test_decode_plans_and_refusals(lib):
+    ws = lib.blackflash_decode_workspace_bytes
+    assert ws(1, 8, 2, 1, 0, 64, 64, 64, 0) == 0          # one split: no workspace
+    assert ws(1, 8, 2, 1, 0, 100000, 64, 512, 4) > 0
+    # The plan follows the window, not the capacity.
+    assert ws(1, 8, 2, 1, 0, 1 << 30, 128, 512, 4) == ws(1, 8, 2, 1, 0, 1000, 128, 512, 4)
+    assert ws(64, 32, 8, 1, 16384, 1024, 128, 2 ** 31 - 1, 0) % 4 == 0
+    for bad in ((0, 8, 2, 1, 0, 64, 64, 64, 0), (1, 8, 3, 1, 0, 64, 64, 64, 0), (1, 8, 2, 0, 0, 64, 64, 64, 0),
+                (1, 8, 2, 1, 0, 0, 64, 64, 0), (1, 8, 2, 1, -1, 64, 64, 64, 0), (1, 8, 2, 1, 0, 64, 80, 64, 0),
+                (1, 8, 2, 1, 0, 64, 64, 0, 0), (1, 8, 2, 1, 0, 64, 64, 4, -1), (1, 1 << 20, 1, 2, 0, 64, 64, 4, 0),
+                (65536, 65536, 65536, 1, 0, 64, 64, 4, 0)):
+        assert ws(*bad) == -1 and lib.blackflash_last_error(), bad
+    v = view(lib)
+    need = ws(1, 8, 2, 1, 0, 100000, 64, 5000, 4)
+    sizes = (1, 8, 2, 1, 100000, 64, 5000, 4, 0.125, 0, None)
+    for args, text in (((None, v, v, 16, 16, None, 16, need), b"Q and O"), ((16, v, v, None, 16, None, 16, need), b"lengths"),
+                       ((16, v, v, 16, 16, None, 16, need - 1), b"workspace"), ((16, v, v, 16, 16, None, None, need), b"workspace"),
+                       ((16, v, v, 16, 16, None, 24, need), b"workspace"), ((16, None, v, 16, 16, None, 16, need), b"K_cache")):
+        assert lib.blackflash_window_decode(*args, *sizes) == 1
+        assert text in lib.blackflash_last_error()
+    big = 1 << 30
+    p = (1, 8, 2, 1, 100, 50, 64)
+    for args, text in (((16, None, v, v, v, 16, 16, None, 16, big), b"prefix"), ((16, v, v, v, None, 16, 16, None, 16, big), b"V_cache"),
+                       ((16, v, v, v, v, 16, 16, None, None, big), b"workspace")):
+        assert lib.blackflash_prefix_decode(*args, *p, 0.125, 0, None) == 1
+        assert text in lib.blackflash_last_error()
+    assert lib.blackflash_prefix_decode(16, v, v, v, v, 16, 16, None, 16, big, *p, math.inf, 0, None) == 1
+
+
+def test_rotary_refusals(lib):
+    v = view(lib)
+    ok = dict(B=1, Hq=2, Hk=1, N=3, d=64, rot=64, inter=0, amp=1.0, inv=0, dtype=0)
+    for change in (dict(B=0), dict(N=0), dict(Hq=0, Hk=0), dict(Hq=-1), dict(Hq=70000), dict(d=65), dict(d=2048),
+                   dict(rot=0), dict(rot=66), dict(rot=7), dict(amp=math.inf), dict(dtype=3)):
+        a = {**ok, **change}
+        assert lib.blackflash_rotary(v, v, 16, 16, 16, 0, 0, 16, *a.values(), None) == 1, change
+        assert lib.blackflash_last_error()
+    for args in ((None, v, 16, 16, 16, 0, 0, 16), (v, v, None, 16, 16, 0, 0, 16), (v, v, 16, 16, None, 0, 0, 16),
+                 (v, v, 16, 16, 16, 0, 0, None), (view(lib, data=18), v, 16, 16, 16, 0, 0, 16), (v, v, 16, 18, 16, 0, 0, 16),
+                 (view(lib, strides=(64, 63, 64)), v, 16, 16, 16, 0, 0, 16), (view(lib, strides=(64, -64, 64)), v, 16, 16, 16, 0, 0, 16)):
+        assert lib.blackflash_rotary(*args, *ok.values(), None) == 1
+        assert lib.blackflash_last_error()
+
+
+def test_python_checks():
+    import blackflash_b200 as bf
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t)  # noqa: E731
+    q, n = z(1, 2, 4, 64), torch.zeros(1, dtype=torch.int32)
+    f = torch.zeros(32, dtype=torch.float64)
+    for call in (lambda: bf.window_attention(q, q, q, 4), lambda: bf.window_attention(q.float(), q, q, 4),
+                 lambda: bf.window_attention_lse(None, q, q, 4), lambda: bf.window_decode(q, q, q, n, 4),
+                 lambda: bf.prefix_decode(q, q[0], q[0], q, q, n), lambda: bf.rotary(q, q, n, f)):
+        with pytest.raises(RuntimeError, match="must be a"):
+            call()
+    for kw in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=4, base=1.0), dict(rotary_dim=4, factor=0.5),
+               dict(rotary_dim=4, scaling="cubic"), dict(rotary_dim=2, scaling="ntk", factor=2.0),
+               dict(rotary_dim=4, scaling="by-parts", factor=2.0)):
+        with pytest.raises(RuntimeError):
+            bf.rotary_frequencies(**kw, device="cpu")
+
+
+def test_rotary_frequency_scalings():
+    from blackflash_b200 import rotary_frequencies
+    f, a = rotary_frequencies(64, 10000.0, device="cpu")
+    assert a == 1.0 and f.dtype == torch.float64 and f[0] == 1.0 and abs(f[1] / 10000 ** (-1 / 32) - 1) < 1e-15
+    assert torch.equal(rotary_frequencies(64, 10000.0, "linear", 8.0, device="cpu")[0], f / 8)
+    g, _ = rotary_frequencies(64, 10000.0, "ntk", 8.0, device="cpu")
+    assert g[0] == 1.0 and abs(g[-1] * 8 / f[-1] - 1) < 1e-12
+    g, a = rotary_frequencies(64, 10000.0, "by-parts", 8.0, 4096, device="cpu")
+    assert torch.equal(g[:5], f[:5]) and torch.allclose(g[-5:], f[-5:] / 8, rtol=1e-14, atol=0)
+    assert (g[1:] < g[:-1]).all() and abs(a - (1 + 0.1 * math.log(8))) < 1e-15
