@@ -32,6 +32,8 @@ EXPORTED = (
     "blackflash_ring_status",
     "blackflash_ring_destroy",
     "blackflash_window_fwd",
+    "blackflash_window_bwd",
+    "blackflash_window_bwd_workspace_bytes",
     "blackflash_decode_workspace_bytes",
     "blackflash_window_decode",
     "blackflash_prefix_decode",
@@ -81,6 +83,8 @@ _SIGS = {
     "blackflash_fwd_debug_s": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp]),
     "blackflash_fwd_trace": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "blackflash_window_fwd": (_i, [_view] * 3 + [_vp, _vp] + [_i] * 8 + [_f, _i, _vp]),
+    "blackflash_window_bwd": (_i, [_view] * 3 + [_vp, _view] + [_vp] * 5 + [_ll] + [_i] * 8 + [_f, _vp]),
+    "blackflash_window_bwd_workspace_bytes": (_ll, [_i] * 8),
     "blackflash_decode_workspace_bytes": (_ll, [_i] * 9),
     "blackflash_window_decode": (_i, [_vp, _view, _view, _vp, _vp, _vp, _vp, _ll] + [_i] * 8 + [_f, _i, _vp]),
     "blackflash_prefix_decode": (_i, [_vp] + [_view] * 4 + [_vp, _vp, _vp, _vp, _ll] + [_i] * 7 + [_f, _i, _vp]),

@@ -24,7 +24,7 @@ EXT_SRC = os.path.join(CSRC, "torch_ext.cpp")
 SOURCES = ["fa_fwd_sm100.cu", "capi.cu", "lse_merge.cu", "noalloc.cu", "ring_ipc.cu", "window_sm100.cu", "decode.cu",
            "rotary.cu"]
 HEADERS = ["sm100_ptx.cuh", "fa_fwd_sm100.h", "fa_fwd_sm100_d128.cuh", "fa_bwd_sm100.cuh", "launch_sm100.h", "views.h",
-           "window_fwd_sm100.cuh"]
+           "window_fwd_sm100.cuh", "window_bwd_sm100.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", os.path.join(REPO_DIR, "include")]
 

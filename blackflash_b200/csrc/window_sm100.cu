@@ -18,6 +18,7 @@ __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
 }
 
 #include "window_fwd_sm100.cuh"
+#include "window_bwd_sm100.cuh"
 
 }  // namespace bfk
 
@@ -109,6 +110,161 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
     if ((rc = make_map_4d(&mk, K->data, f16, dk, tk, 128, 1)) != BF_OK) return rc;
     if ((rc = make_map_4d(&mv, V->data, f16, dk, tv, 128, 1)) != BF_OK) return rc;
     return launch_fwd<false>(d, f16, mq, mk, mv, p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+// How the dK/dV pass is split, and its workspace: -lse2 and -D, then the parts.
+struct BwdPlan {
+    int nk, ns, window, sinks, n_pad, splits_s, splits_n;
+    long long vec, slots, bytes;
+};
+
+BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks) {
+    BwdPlan p;
+    p.window = window < Nkv ? window : Nkv;
+    p.sinks = sinks < Nkv ? sinks : Nkv;
+    p.nk = (Nkv + 127) / 128;
+    p.ns = (p.sinks + 127) / 128;
+    p.n_pad = (Nq + 127) / 128 * 128;
+    const int nt = d == 64 ? 128 : 64;
+    const long long units = (long long)B * Hkv, group = Hq / Hkv;
+    // Steps of a tile that only its window's queries see, and of one that holds sinks.
+    const long long seen = (long long)p.window + 127 < Nq ? (long long)p.window + 127 : Nq;
+    const long long norm = group * ((seen + nt - 1) / nt), sink = group * ((Nq + nt - 1) / nt);
+    const long long total = units * ((p.nk - p.ns) * norm + p.ns * sink);
+    // Two items a multiprocessor where the work allows it, none shorter than 16 steps (below
+    // that a part's own fp32 output weighs more than what it reads); a sink tile in parts no
+    // shorter than the other items.
+    long long target = (total + 2 * kPlanSms - 1) / (2 * kPlanSms);
+    if (target < 16) target = 16;
+    p.splits_n = norm * 2 > target * 3 ? (int)((norm + target - 1) / target) : 1;
+    const long long target_s = target > norm ? target : norm;
+    p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
+    p.vec = (long long)B * Hq * p.n_pad;
+    p.slots = units * ((p.splits_s > 1 ? (long long)p.ns * p.splits_s : 0) +
+                       (p.splits_n > 1 ? (long long)(p.nk - p.ns) * p.splits_n : 0));
+    p.bytes = 4 * (2 * p.vec + p.slots * 2 * 128 * d);
+    return p;
+}
+
+template <int D, bool kDQ>
+int launch_bwd(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0, const CUtensorMap& y1,
+               const bfk::winb::Params& p, cudaStream_t stream) {
+    static std::atomic<bool> done[64];  // per device; zero-initialised (static storage)
+    auto kernel = bfk::winb::window_bwd_kernel<D, kDQ>;
+    int rc, sms = 0;
+    if ((rc = allow_smem(kernel, bfk::winb::smem_bytes<D, kDQ>(), done)) != BF_OK) return rc;
+    if ((rc = sm_count(&sms)) != BF_OK) return rc;
+    const int grid = p.items < sms ? p.items : sms;  // persistent: one block per multiprocessor
+    return launch_error(launch_pdl(kernel, dim3((unsigned)grid), bfk::winb::kThreads, bfk::winb::smem_bytes<D, kDQ>(),
+                                   stream, x0, x1, y0, y1, p));
+}
+
+}  // namespace
+
+extern "C" long long blackflash_window_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window,
+                                                           int sinks) {
+    bf_set_error(BF_OK, "");
+    if (check_window(B, Hq, Hkv, Nq, Nkv, d, window, sinks, 1.f) != BF_OK) return -1;
+    return bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks).bytes;
+}
+
+extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, const void* O, const bf_view* dO,
+                                     const float* lse, void* dQ, void* dK, void* dV, void* workspace,
+                                     long long workspace_bytes, int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window,
+                                     int sinks, float scale, void* stream) {
+    bf_set_error(BF_OK, "");
+    int rc;
+    if ((rc = check_window(B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale)) != BF_OK) return rc;
+    ViewStrides sq, sk, sv, sd;
+    if ((rc = check_view(Q, "Q", B, Hq, Nq, d, 2, &sq)) != BF_OK) return rc;
+    if ((rc = check_view(K, "K", B, Hkv, Nkv, d, 2, &sk)) != BF_OK) return rc;
+    if ((rc = check_view(V, "V", B, Hkv, Nkv, d, 2, &sv)) != BF_OK) return rc;
+    if ((rc = check_view(dO, "dO", B, Hq, Nq, d, 2, &sd)) != BF_OK) return rc;
+    const void* ptrs[] = {O, dQ, dK, dV, workspace};
+    for (const void* ptr : ptrs)
+        if (!ptr || (reinterpret_cast<uintptr_t>(ptr) & 15u))
+            return bf_set_error(BF_ERR_ARG, "O, dQ, dK, dV and the workspace must be non-null and 16-byte aligned");
+    if (!lse) return bf_set_error(BF_ERR_ARG, "lse: null pointer");
+    const BwdPlan plan = bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks);
+    if (workspace_bytes < plan.bytes)
+        return bf_set_error(BF_ERR_ARG, "workspace smaller than blackflash_window_bwd_workspace_bytes()");
+    const int nt = d == 64 ? 128 : 64;
+    const int q_tiles = plan.n_pad / 128;
+    const long long units = (long long)B * Hkv;
+    const long long kv_items = units * ((long long)plan.ns * plan.splits_s + (long long)(plan.nk - plan.ns) * plan.splits_n);
+    const long long q_items = (long long)B * Hq * q_tiles;
+    if ((long long)B * Hq > 0x7fffffffLL || kv_items > 0x7fffffffLL || q_items > 0x7fffffffLL ||
+        (long long)(Hq / Hkv) * (plan.n_pad / nt) > 0x7fffffffLL || plan.vec / 8 > 0x7fffffffLL)
+        return bf_set_error(BF_ERR_ARG, "problem too large for one launch");
+
+    if ((rc = bind_context()) != BF_OK) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    float* nlse2 = reinterpret_cast<float*>(workspace);
+    float* nd = nlse2 + plan.vec;
+    float* part = nd + plan.vec;
+    {
+        const int per = 256 / (d / 8);
+        const unsigned grid = (unsigned)((plan.vec + per - 1) / per);
+        auto kernel = d == 64 ? bfk::winb::prep_kernel<64> : bfk::winb::prep_kernel<128>;
+        if ((rc = launch_error(launch_pdl(kernel, dim3(grid), 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
+                                          reinterpret_cast<const char*>(dO->data), sd.s[0] * 2, sd.s[1] * 2, sd.s[2] * 2, lse,
+                                          nlse2, nd, Hq, Nq, plan.n_pad, plan.vec))) != BF_OK)
+            return rc;
+    }
+    const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
+    const long long tq[3] = {sq.s[2], sq.s[1], sq.s[0]}, tk[3] = {sk.s[2], sk.s[1], sk.s[0]},
+                    tv[3] = {sv.s[2], sv.s[1], sv.s[0]}, td[3] = {sd.s[2], sd.s[1], sd.s[0]};
+    CUtensorMap mq, mk, mv, md, sq_map, sd_map;  // 128-row boxes; streamed queries in nt-row boxes
+    if ((rc = make_map_4d(&mq, Q->data, false, dq, tq, 128, 1)) != BF_OK) return rc;
+    if ((rc = make_map_4d(&md, dO->data, false, dq, td, 128, 1)) != BF_OK) return rc;
+    if ((rc = make_map_4d(&mk, K->data, false, dk, tk, 128, 1)) != BF_OK) return rc;
+    if ((rc = make_map_4d(&mv, V->data, false, dk, tv, 128, 1)) != BF_OK) return rc;
+    if ((rc = make_map_4d(&sq_map, Q->data, false, dq, tq, nt, 1)) != BF_OK) return rc;
+    if ((rc = make_map_4d(&sd_map, dO->data, false, dq, td, nt, 1)) != BF_OK) return rc;
+
+    bfk::winb::Params p;
+    memset(&p, 0, sizeof(p));
+    p.batch = B;
+    p.hq = Hq;
+    p.hkv = Hkv;
+    p.group = Hq / Hkv;
+    p.n_q = Nq;
+    p.n_kv = Nkv;
+    p.n_pad = plan.n_pad;
+    p.nk = plan.nk;
+    p.ns = plan.ns;
+    p.window = plan.window;
+    p.sinks = plan.sinks;
+    p.q_tiles = q_tiles;
+    p.splits_s = plan.splits_s;
+    p.splits_n = plan.splits_n;
+    p.scale = scale;
+    p.scale_log2 = scale * kLog2e;
+    p.nlse2 = nlse2;
+    p.nd = nd;
+    p.dq = reinterpret_cast<__nv_bfloat16*>(dQ);
+    p.dk = reinterpret_cast<__nv_bfloat16*>(dK);
+    p.dv = reinterpret_cast<__nv_bfloat16*>(dV);
+    p.part = part;
+    p.timeout_ns = kTimeoutNs;
+    p.items = (int)kv_items;
+    rc = d == 64 ? launch_bwd<64, false>(mk, mv, sq_map, sd_map, p, st) : launch_bwd<128, false>(mk, mv, sq_map, sd_map, p, st);
+    if (rc != BF_OK) return rc;
+    auto join = [&](const float* from, int j0, int tiles, int splits) -> int {
+        if (splits <= 1 || tiles <= 0) return BF_OK;
+        const long long threads = units * tiles * 2 * 128 * (d / 4);
+        if (threads / 256 >= 0x7fffffffLL) return bf_set_error(BF_ERR_ARG, "problem too large for one launch");
+        auto kernel = d == 64 ? bfk::winb::join_kernel<64> : bfk::winb::join_kernel<128>;
+        return launch_error(launch_pdl(kernel, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, from, p.dk, p.dv, j0, tiles,
+                                       splits, Nkv, units));
+    };
+    if ((rc = join(part, 0, plan.ns, plan.splits_s)) != BF_OK) return rc;
+    const float* rest = part + (plan.splits_s > 1 ? units * plan.ns * plan.splits_s * 2 * 128 * d : 0);
+    if ((rc = join(rest, plan.ns, plan.nk - plan.ns, plan.splits_n)) != BF_OK) return rc;
+    p.items = (int)q_items;
+    return d == 64 ? launch_bwd<64, true>(mq, md, mk, mv, p, st) : launch_bwd<128, true>(mq, md, mk, mv, p, st);
 }
 
 int bf_prefix_partial(const PrefixArgs& a) {

@@ -99,6 +99,61 @@ def window_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, window: 
     return window_attention_lse(Q, K, V, window, sinks, scale, want_lse=False)[0]
 
 
+def window_attention_backward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.Tensor, dO: torch.Tensor,
+                              lse: torch.Tensor, window: int, sinks: int = 0, scale: float | None = None):
+    """Gradients (dQ, dK, dV) of `window_attention` for upstream dO; bf16.
+
+    O and lse as `window_attention_lse` returned them; dO [B, Hq, Nq, d] may be a strided
+    view. dK and dV are summed over the query heads that share a KV head."""
+    _check_grouped(Q, K, V)
+    _require(Q.dtype == torch.bfloat16, "the backward supports bfloat16")
+    window, sinks = _check_window(window, sinks)
+    scale = _check_scale(scale, Q.size(3))
+    _check("O", O, 4, Q)
+    _check("dO", dO, 4, Q)
+    _require(O.shape == Q.shape and dO.shape == Q.shape and O.is_contiguous(), "O must be contiguous, O and dO of Q's shape")
+    _require(isinstance(lse, torch.Tensor) and lse.dtype == torch.float32 and lse.device == Q.device
+             and lse.is_contiguous() and lse.shape == Q.shape[:3], "lse must be a contiguous fp32 [B, Hq, Nq] tensor")
+    B, Hq, Nq, d = Q.shape
+    Hkv, Nkv = K.size(1), K.size(2)
+    dQ, dK, dV = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (Q, K, V))
+    if Q.numel() == 0 or K.numel() == 0:
+        return dQ.zero_(), dK.zero_(), dV.zero_()
+    lib = _lib.load()
+    with torch.cuda.device(Q.device):
+        nbytes = lib.blackflash_window_bwd_workspace_bytes(B, Hq, Hkv, Nq, Nkv, d, window, sinks)
+        if nbytes < 0:
+            _lib.check(_lib.BF_ERR_ARG, "blackflash_window_bwd_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        rc = lib.blackflash_window_bwd(
+            _view(Q), _view(K), _view(V), O.data_ptr(), _view(dO), lse.data_ptr(), dQ.data_ptr(), dK.data_ptr(),
+            dV.data_ptr(), ws.data_ptr(), nbytes, B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale, _stream_handle(Q.device))
+    _lib.check(rc, "blackflash_window_bwd")
+    return dQ, dK, dV
+
+
+class _WindowFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, Q, K, V, window, sinks, scale):
+        O, lse = window_attention_lse(Q, K, V, window, sinks, scale)
+        ctx.save_for_backward(Q, K, V, O, lse)
+        ctx.args = (window, sinks, scale)
+        return O
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dO):
+        Q, K, V, O, lse = ctx.saved_tensors
+        return (*window_attention_backward(Q, K, V, O, _rows(dO), lse, *ctx.args), None, None, None)
+
+
+def window_attention_with_grad(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, window: int, sinks: int = 0,
+                               scale: float | None = None) -> torch.Tensor:
+    """`window_attention` as a differentiable op; bf16."""
+    _require(Q.dtype == torch.bfloat16, "the backward supports bfloat16")
+    return _WindowFn.apply(Q, K, V, window, sinks, scale)
+
+
 # ---------------------------------------------------------------- decoding steps
 
 def _check_step(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lengths: torch.Tensor) -> None:

@@ -182,6 +182,19 @@ int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const bf_view* V, 
                           int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale, int dtype, void* stream);
 
 /*
+ * Gradients of blackflash_window_fwd for an upstream dO [B, Hq, Nq, d], bf16. O contiguous and
+ * lse [B, Hq, Nq] as the forward wrote them; dQ [B, Hq, Nq, d] and dK, dV [B, Hkv, Nkv, d]
+ * contiguous, summed over the query heads that share a KV head. Rows that see nothing, and
+ * keys that nothing sees, get zeros. The result does not depend on scheduling: no atomics.
+ *   workspace: device memory of blackflash_window_bwd_workspace_bytes(...) bytes (-1 for bad
+ *   sizes), 16-byte aligned, overwritten. Calls that overlap on the GPU need their own.
+ */
+long long blackflash_window_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks);
+int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, const void* O, const bf_view* dO,
+                          const float* lse, void* dQ, void* dK, void* dV, void* workspace, long long workspace_bytes, int B,
+                          int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale, void* stream);
+
+/*
  * Decoding steps: T >= 1 new tokens of each sequence against its cache. No counterpart in
  * the reference.
  *   Q: [B, Hq, T, d] contiguous; K, V: caches [B, Hkv, C, d] of any strides; lengths: [B]

@@ -68,6 +68,38 @@ def window_ref(q, k, v, window, sinks, scale):
     return o, lse, pv
 
 
+def window_grad_ref(q, k, v, do, window, sinks, scale):
+    """Gradients in fp64 and the elementwise bound of each.
+
+    With h half a bf16 step and e = EXP_REL: P enters dV rounded (h) and off by e; dS is
+    P (dP - D), off by e of itself, by P times D's error, and rounded (h). D comes from the
+    rounded O, itself within o_bound, so its error is sum |dO| o_bound. Each gradient is
+    rounded once more (h)."""
+    b, hq, nq, d = q.shape
+    hkv = k.shape[1]
+    g = hq // hkv
+    h = half_step(torch.bfloat16)
+    q6, do6 = q.double(), do.double()
+    k6, v6 = (x.double().repeat_interleave(g, 1) for x in (k, v))
+    seen = visible(nq, k.shape[2], window, sinks, q.device)
+    o, _, p, pv = attention64(q6, k6, v6, seen, scale)
+    dv = p.transpose(-1, -2) @ do6
+    dp = do6 @ v6.transpose(-1, -2)
+    ds = p * (dp - (do6 * o).sum(-1, keepdim=True)) * scale
+    d_err = (do6.abs() * o_bound(o, pv, torch.bfloat16)).sum(-1, keepdim=True)
+    # dP itself is an fp32 sum of d exact products: d steps of the sum of their sizes.
+    dp_err = d * 2.0 ** -24 * (do6.abs() @ v6.abs().transpose(-1, -2))
+    e_ds = (h + EXP_REL) * (ds.abs() + p * scale * (d_err + dp_err)) + p * scale * (d_err + dp_err)
+    grads = {"dq": ds @ k6, "dk": ds.transpose(-1, -2) @ q6, "dv": dv}
+    errs = {"dq": e_ds @ k6.abs(), "dk": e_ds.transpose(-1, -2) @ q6.abs(),
+            "dv": (h + EXP_REL) * (p.transpose(-1, -2) @ do6.abs())}
+    for x in ("dk", "dv"):
+        grads[x] = grads[x].view(b, hkv, g, *grads[x].shape[2:]).sum(2)
+        errs[x] = errs[x].view(b, hkv, g, *errs[x].shape[2:]).sum(2)
+    # 1e-5 of the terms' size for fp32 sums over some thousand of them.
+    return {x: (grads[x], errs[x] * (1 + 1e-5) + h * grads[x].abs() + 1e-6) for x in grads}
+
+
 def decode_ref(q, k, v, lengths, window, sinks, scale, kp=None, vp=None):
     """Sequence by sequence; kp, vp [Hkv, P, d] are seen by every token."""
     b, hq, t, d = q.shape

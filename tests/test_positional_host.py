@@ -18,7 +18,31 @@ def lib():
     from blackflash_b200 import _lib
     from blackflash_b200.build import build_lib
     build_lib()
-    return _lib.load()
+    yield _lib.load()
+    _lib.load().blackflash_decode_workspace_bytes(1, 1, 1, 1, 0, 1, 64, 1, 0)  # clears the thread's last error
+
+
+@pytest.mark.parametrize("change", [dict(B=0), dict(Hkv=3), dict(d=32), dict(window=0), dict(sinks=-2)])
+def test_window_backward_plans(lib, change):
+    ok = dict(B=1, Hq=4, Hkv=2, Nq=300, Nkv=300, d=64, window=50, sinks=0)
+    ws = lib.blackflash_window_bwd_workspace_bytes
+    assert ws(*ok.values()) == 4 * 2 * 4 * 384            # two vectors of 4 heads, 300 rows padded to 384
+    # Sinks that 100 query tiles see come in parts: 128-row fp32 pieces of dV and dK.
+    many = ws(*{**ok, "Nq": 12800, "Nkv": 12800, "sinks": 4}.values()) - 4 * 2 * 4 * 12800
+    assert many > 0 and many % (2 * 128 * 64 * 4) == 0
+    assert ws(*{**ok, **change}.values()) == -1 and lib.blackflash_last_error()
+
+
+def test_window_backward_refusals(lib):
+    ok, sizes = view(lib), (1, 2, 2, 8, 8, 64, 4, 0, 0.125, None)
+    need = lib.blackflash_window_bwd_workspace_bytes(*sizes[:8])
+    good = [ok, ok, ok, 16, ok, 16, 16, 16, 16, 16, need]
+    for i, bad, text in ((0, None, b"Q:"), (4, view(lib, strides=(64, 3, 64)), b"dO"), (3, None, b"O, dQ"), (5, None, b"lse"),
+                         (8, 24, b"O, dQ"), (9, None, b"workspace"), (10, need - 1, b"workspace")):
+        args = list(good)
+        args[i] = bad
+        assert lib.blackflash_window_bwd(*args, *sizes) == 1 and text in lib.blackflash_last_error()
+    assert lib.blackflash_window_bwd(*good, *sizes[:8], -1.0, None) == 1
 
 
 WINDOW = dict(B=1, Hq=2, Hkv=1, Nq=8, Nkv=8, d=64, window=4, sinks=0, scale=0.125, dtype=0)

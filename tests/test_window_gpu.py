@@ -133,3 +133,127 @@ def test_window_nan_query_row_stays_its_own():
     assert torch.isnan(got[0, 1, 150]).all()
     got[0, 1, 150] = want[0, 1, 150]
     assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------- gradients
+
+def check_grads(got, q, k, v, do, window, sinks, scale=None):
+    scale = 1 / math.sqrt(q.shape[3]) if scale is None else scale
+    want = ref.window_grad_ref(q, k, v, do, window, sinks, scale)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        g, lim = want[name]
+        err = (x.double() - g).abs()
+        bad = int((err > lim).sum())
+        assert bad == 0 and torch.isfinite(x).all(), (name, bad, x.numel(), float((err / lim).max()))
+
+
+def grads_of(q, k, v, do, window, sinks, scale=None):
+    from blackflash_b200 import wait_status, window_attention_backward, window_attention_lse
+    o, lse = window_attention_lse(q, k, v, window, sinks, scale)
+    got = window_attention_backward(q, k, v, o, do, lse, window, sinks, scale)
+    torch.cuda.synchronize()
+    assert wait_status() == 0
+    return got
+
+
+def upstream(q, seed=1):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(q.shape, generator=gen, device="cuda").to(q.dtype)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq,nkv,window,sinks", [
+    (1, 1, 1, 0), (3, 3, 2, 1), (64, 64, 64, 0), (65, 65, 10, 2), (128, 128, 128, 0), (129, 129, 1, 0), (255, 255, 64, 4),
+    (300, 300, 129, 1), (640, 640, 127, 129), (1000, 1000, 100, 300), (1000, 1000, 5000, 0), (777, 777, 1, 4),
+    (1, 700, 50, 3), (130, 1000, 200, 16), (300, 100, 20, 2), (600, 1, 4, 0), (2500, 2500, 64, 4),
+])
+def test_window_backward_parity(d, nq, nkv, window, sinks):
+    q, k, v = make(2, 4, 2, nq, nkv, d, seed=nq + nkv)
+    do = upstream(q)
+    check_grads(grads_of(q, k, v, do, window, sinks), q, k, v, do, window, sinks)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (3, 1), (8, 1), (10, 5)])
+def test_window_backward_head_groups_and_views(hq, hkv):
+    for d in (64, 128):
+        q, k, v = make(2, hq, hkv, 333, 461, d, seed=hq, heads_last=True)
+        do = upstream(q.transpose(1, 2)).transpose(1, 2)
+        check_grads(grads_of(q, k, v, do, 150, 5), q, k, v, do, 150, 5)
+
+
+def test_window_backward_many_items_and_parts():
+    """More items than multiprocessors, sink tiles in many parts, and a second run bit for bit."""
+    for d, hq, hkv, n, w, s in ((64, 8, 2, 2000, 200, 4), (128, 8, 2, 2000, 200, 140), (64, 16, 16, 1300, 100, 1)):
+        q, k, v = make(3, hq, hkv, n, n, d, seed=d)
+        do = upstream(q)
+        got = grads_of(q, k, v, do, w, s)
+        check_grads(got, q, k, v, do, w, s)
+        for a, b in zip(got, grads_of(q, k, v, do, w, s)):
+            assert torch.equal(a, b)
+
+
+def test_window_autograd_broadcast_and_differences():
+    """Through autograd: K and V shared by expansion, a broadcast upstream, and a difference."""
+    from blackflash_b200 import window_attention, window_attention_with_grad
+    q, k, v = make(2, 4, 1, 300, 300, 64, seed=11)
+    do = upstream(q)
+    a = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    got = torch.autograd.grad(window_attention_with_grad(*a, 90, 4), a, do)
+    check_grads(got, q, k, v, do, 90, 4)
+    # One K/V head for all batches: the expanded leaf gets the sum over the batch.
+    leaf = k[:1].clone().requires_grad_(True)
+    kk = leaf.expand(2, 1, 300, 64).contiguous()
+    g, = torch.autograd.grad(window_attention_with_grad(q, kk, v, 90, 4), leaf, do)
+    full = torch.autograd.grad(window_attention_with_grad(q, kk, v, 90, 4), kk, do)[0]
+    assert torch.equal(g, full.sum(0, keepdim=True))
+    # A sum's gradient is one expanded number.
+    x = q.clone().requires_grad_(True)
+    g, = torch.autograd.grad(window_attention_with_grad(x, k, v, 90, 4).sum(), x)
+    check_grads((g,), q, k, v, torch.ones_like(q), 90, 4)
+    # A difference along a direction of V, in which O is linear: <dO, O(V + e) - O(V)> = <dV, e>.
+    e = upstream(v, 5)
+    v2 = (v + e).to(v.dtype)
+    e = v2.double() - v.double()
+    left = (do.double() * (window_attention(q, k, v2, 90, 4).double() - window_attention(q, k, v, 90, 4).double())).sum()
+    right = (got[2].double() * e).sum()
+    # Both sides are sums of 76800 and 38400 rounded terms; each term's bound adds up, in size.
+    o1, _, pv1 = ref.window_ref(q, k, v, 90, 4, 0.125)
+    o2, _, pv2 = ref.window_ref(q, k, v2, 90, 4, 0.125)
+    lim = (do.double().abs() * (ref.o_bound(o1, pv1, q.dtype) + ref.o_bound(o2, pv2, q.dtype))).sum()
+    lim = lim + (ref.window_grad_ref(q, k, v, do, 90, 4, 0.125)["dv"][1] * e.abs()).sum()
+    assert abs(left - right) <= lim
+
+
+def test_window_training_step_in_a_graph():
+    """Forward and backward captured, replayed on new data, on a stream of their own."""
+    from blackflash_b200 import window_attention_with_grad
+    q, k, v = (x.requires_grad_(True) for x in make(1, 4, 2, 300, 300, 128, seed=12))
+    do = upstream(q)
+
+    def step():
+        o = window_attention_with_grad(q, k, v, 100, 4)
+        return (o.detach(), *torch.autograd.grad(o, (q, k, v), do))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    with torch.no_grad():
+        for x, y in zip((q, k, v), make(1, 4, 2, 300, 300, 128, seed=13)):
+            x.copy_(y)
+    want = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+        assert torch.equal(a, b)
+
+
+def test_window_backward_empty():
+    from blackflash_b200 import window_attention_backward
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    q, k = z(2, 4, 3, 64), z(2, 2, 0, 64)
+    dq, dk, dv = window_attention_backward(q, k, k, q, q, torch.zeros(2, 4, 3, device="cuda"), 5)
+    assert (dq == 0).all() and dk.shape == dv.shape == k.shape
