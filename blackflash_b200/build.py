@@ -20,6 +20,8 @@ HARNESS_PATH = os.path.join(LIB_DIR, "flash_attn")
 # The torch-extension module `blackflash_cuda`, built at the repository root so that
 # `import blackflash_cuda` resolves as it does for the reference's installed extension.
 EXT_SRC = os.path.join(CSRC, "torch_ext.cpp")
+# The torch binding of the position-aware operators, `blackflash_b200._positional`.
+POSITIONAL_SRC = os.path.join(CSRC, "torch_positional.cpp")
 
 SOURCES = ["fa_fwd_sm100.cu", "capi.cu", "lse_merge.cu", "noalloc.cu", "ring_ipc.cu", "window_sm100.cu", "decode.cu",
            "rotary.cu"]
@@ -84,16 +86,20 @@ def ext_path() -> str:
     return os.path.join(REPO_DIR, "blackflash_cuda" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
-    """Compile the `blackflash_cuda` torch extension (csrc/torch_ext.cpp, g++ against the
-    installed torch headers) linked to libblackflash_b200.so; return its path."""
+def positional_path() -> str:
+    import sysconfig
+    return os.path.join(PKG_DIR, "_positional" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _build_ext(name: str, src: str, out: str, rpath: str, force: bool, verbose: bool) -> str:
+    """Compile a torch extension (g++ against the installed torch headers) linked to
+    libblackflash_b200.so, found at run time at `rpath`; return its path."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
     lib = build_lib(force=force, verbose=verbose)
-    out = ext_path()
-    deps = [EXT_SRC, lib, os.path.join(REPO_DIR, "include", "blackflash_b200.h")]
+    deps = [src, lib, os.path.join(REPO_DIR, "include", "blackflash_b200.h")]
     if not (force or _stale(out, deps)):
         return out
     cuda_home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
@@ -103,14 +109,21 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     abi = int(torch.compiled_with_cxx11_abi())
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-DTORCH_EXTENSION_NAME=blackflash_cuda",
-           *[f"-I{i}" for i in incs], EXT_SRC, "-o", out + ".tmp",
-           f"-L{LIB_DIR}", "-lblackflash_b200", "-Wl,-rpath,$ORIGIN/blackflash_b200/lib",
+           f"-DTORCH_EXTENSION_NAME={name}",
+           *[f"-I{i}" for i in incs], src, "-o", out + ".tmp",
+           f"-L{LIB_DIR}", "-lblackflash_b200", f"-Wl,-rpath,{rpath}",
            f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            ]
     _run(cmd, verbose)
     os.replace(out + ".tmp", out)
     return out
+
+
+def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
+    """Compile the torch extensions: `blackflash_b200._positional` (csrc/torch_positional.cpp)
+    and `blackflash_cuda` (csrc/torch_ext.cpp); return the latter's path."""
+    _build_ext("_positional", POSITIONAL_SRC, positional_path(), "$ORIGIN/lib", force, verbose)
+    return _build_ext("blackflash_cuda", EXT_SRC, ext_path(), "$ORIGIN/blackflash_b200/lib", force, verbose)
 
 
 if __name__ == "__main__":

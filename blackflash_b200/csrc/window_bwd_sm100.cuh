@@ -17,6 +17,11 @@
 //                    X0  X1   Y0  Y1    S = X0 Y0^T   dP = X1 Y1^T   accumulators
 //   dK/dV (kDQ=0)    K   V    Q   dO    (S^T)         (dP^T)         dV += P^T Y1, dK += dS^T Y0
 //   dQ    (kDQ=1)    Q   dO   K   V                                  dQ += dS Y0
+// D. Both passes read it from an array that the prep kernel fills from O. O is rounded to
+// bf16, and for a row that sees few keys that error is not small against dP - D, of which D
+// is then a large part (one key: dP - D is 0). So with few keys (two_sweeps) the dQ pass
+// walks its KV tiles twice: first it sums P dP and P in fp32, D = sum P dP / sum P, which it
+// also leaves in the array for the dK/dV pass; then it accumulates.
 // Roles: eight elementwise warps (two threads per row), a TMA producer, an issuer of S and
 // dP, an issuer of the accumulations; persistent blocks, so an item's tail overlaps the next
 // one's first products. S has two buffers: S of step n + 1 is computed while the elementwise
@@ -100,7 +105,8 @@ struct Params {
     int splits_s, splits_n;  // dK/dV: parts of a sink tile's and of another tile's queries
     float scale, scale_log2;
     const float* nlse2;      // [B Hq, n_pad] -lse log2(e); -inf past n_q and for rows that see nothing
-    const float* nd;         // [B Hq, n_pad] -D
+    float* nd;               // [B Hq, n_pad] -D
+    int two_sweeps;          // dQ: find D in a first sweep over the KV tiles, and store it
     __nv_bfloat16 *dq, *dk, *dv;
     float* part;             // [slot][dV, dK][128][D] of the tiles with more than one part
     unsigned long long timeout_ns;
@@ -109,7 +115,7 @@ struct Params {
 struct Item {
     int b, kvh, head;   // head: the query head (dQ)
     int tile;           // stationary 128-row tile
-    int steps;
+    int steps;          // dQ: of one sweep
     int i0, ni, s0;     // dK/dV: step s is query tile i0 + (s0 + s) % ni of head (s0 + s) / ni
     int n_sink, skip;   // dQ: step s is KV tile s, or s + skip past the sink tiles
     long long slot;     // dK/dV: part to write, -1: the gradient itself
@@ -246,14 +252,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             decode<D, kDQ>(p, item, it);
             const int xrow = it.tile * 128 + row;
             // dQ: the row's -lse2 and -D (padded rows have entries).
+            const int lead = kDQ && p.two_sweeps ? it.steps : 0;  // steps of the first sweep
+            const size_t at = kDQ ? ((size_t)it.b * p.hq + it.head) * p.n_pad + xrow : 0;
             uint64_t nl2 = 0, nd2 = 0;
+            float sum_p = 0.f, sum_pdp = 0.f;
             if constexpr (kDQ) {
-                const size_t at = ((size_t)it.b * p.hq + it.head) * p.n_pad + xrow;
-                const float a = p.nlse2[at], b = p.nd[at];
+                const float a = p.nlse2[at], b = lead ? 0.f : p.nd[at];
                 nl2 = f2_pack(a, a);
                 nd2 = f2_pack(b, b);
             }
-            for (int s_i = 0; s_i < it.steps; ++s_i, ++n) {
+            for (int s_all = 0; s_all < lead + it.steps; ++s_all, ++n) {
+                const bool measure = kDQ && s_all < lead;
+                const int s_i = measure || !kDQ ? s_all : s_all - lead;
+                if (kDQ && lead && s_all == lead) {
+                    // The two halves of the row; a row that sees nothing has D = 0.
+                    sum_p += __shfl_xor_sync(0xffffffffu, sum_p, 16);
+                    sum_pdp += __shfl_xor_sync(0xffffffffu, sum_pdp, 16);
+                    const float b = sum_p != 0.f ? -sum_pdp / sum_p : 0.f;
+                    nd2 = f2_pack(b, b);
+                    if (h == 0) p.nd[at] = b;
+                }
                 const int buf = n & 1;
                 const uint32_t tS = tl + (uint32_t)(buf * NT);
                 // Visible: column c with c < last and (c >= first or c < snk).
@@ -343,14 +361,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float x0, x1, x2, x3;
                         f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), a), x0, x1);
                         f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c + 2]), __uint_as_float(dp[c + 3])), b), x2, x3);
+                        if (kDQ && measure) {  // D is 0 so far: x is dP
+                            const float* q = pr + 32 * i + c;
+                            sum_p += (q[0] + q[1]) + (q[2] + q[3]);
+                            sum_pdp += (q[0] * x0 + q[1] * x1) + (q[2] * x2 + q[3] * x3);
+                        }
                         dsk[16 * i + c / 2] = pack_bf16x2(pr[32 * i + c] * x0, pr[32 * i + c + 1] * x1);
                         dsk[16 * i + c / 2 + 1] = pack_bf16x2(pr[32 * i + c + 2] * x2, pr[32 * i + c + 3] * x3);
                     }
                 }
+                if (!measure) {
 #pragma unroll
-                for (int i = 0; i < NC / 32; ++i)
-                    tmem_st16x32bx2_x16<NC / 2>(tS + (kDQ ? 0 : NT / 2) + 16 * i, dsk + 16 * i);
-                tmem_wait_st();
+                    for (int i = 0; i < NC / 32; ++i)
+                        tmem_st16x32bx2_x16<NC / 2>(tS + (kDQ ? 0 : NT / 2) + 16 * i, dsk + 16 * i);
+                    tmem_wait_st();
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&bars->p_ready[buf]));
@@ -426,7 +451,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ++n_it;
             __syncwarp();
-            for (int s_i = 0; s_i < it.steps; ++s_i, ++n) {
+            const int lead = kDQ && p.two_sweeps ? it.steps : 0;
+            for (int s_all = 0; s_all < lead + it.steps; ++s_all, ++n) {
+                const int s_i = s_all < lead ? s_all : s_all - lead;
                 const uint32_t f = smem_addr(&bars->y_full[st]);
                 if (!(ok = warp_wait(smem_addr(&bars->y_empty[st]), par, ctl, kSiteProdY))) break;
                 if (leader) {
@@ -490,7 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(smem_addr(&bars->x_full), (uint32_t)n_it & 1u, ctl, kSiteFrontX))) break;
                 tc_fence_after();
             }
-            for (int s_i = 0; s_i < it.steps; ++s_i, ++n) {
+            const int lead = kDQ && p.two_sweeps ? it.steps : 0, last = lead + it.steps - 1;
+            for (int s_i = 0; s_i <= last; ++s_i, ++n) {
                 const int buf = n & 1;
                 const uint32_t y_lo = y_lo0 + (uint32_t)(st * 2 * C::kYTile >> 4);
                 const uint32_t tS = tmem + (uint32_t)(buf * NT);
@@ -519,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                        y_lo + (C::kYTile >> 4) + (uint32_t)(kk >> 2) * (C::kYChunk >> 4) + (uint32_t)(kk & 3) * 2,
                                        desc_hi, kIdescS, kk > 0);
                         umma_commit(smem_addr(&bars->dp_full[db]));
-                        if (s_i == it.steps - 1) umma_commit(smem_addr(&bars->x_empty));
+                        if (s_i == last) umma_commit(smem_addr(&bars->x_empty));
                     }
                     __syncwarp();
                 } else {
@@ -528,14 +556,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         !(ok = warp_wait(smem_addr(&bars->acc_free), (uint32_t)(n_it - 1) & 1u, ctl, kSiteAccFree)))
                         break;
                     tc_fence_after();
-                    if (leader) {
+                    if (leader && s_i >= lead) {
                         const uint32_t acc = tmem + C::kColAcc;
 #pragma unroll
                         for (int kk = 0; kk < NT / 16; ++kk)
 #pragma unroll
                             for (int ch = 0; ch < C::kChunks; ++ch) {
                                 const uint32_t off = ch * (C::kYChunk >> 4) + kk * 128;  // 16 rows of 128 bytes
-                                const uint32_t add = (s_i > 0 || kk > 0) ? 1u : 0u;
+                                const uint32_t add = (s_i > lead || kk > 0) ? 1u : 0u;
                                 if constexpr (kDQ) {
                                     umma_ts_lo(acc + ch * 64, tS + kk * 8, y_lo + off, desc_hi, kIdescG, add);
                                 } else {
@@ -543,9 +571,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     umma_ts_lo(acc + D + ch * 64, tS + NT / 2 + kk * 8, y_lo + off, desc_hi, kIdescG, add);
                                 }
                             }
+                    }
+                    if (leader) {
                         umma_commit(smem_addr(&bars->s_free[buf]));
                         umma_commit(smem_addr(&bars->y_empty[st]));
-                        if (s_i == it.steps - 1) umma_commit(smem_addr(&bars->acc_full));
+                        if (s_i == last) umma_commit(smem_addr(&bars->acc_full));
                     }
                     __syncwarp();
                 }
@@ -580,7 +610,7 @@ template <int D>
 __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restrict__ o, const char* __restrict__ dout,
                                                    long long sb, long long sh, long long sn, const float* __restrict__ lse,
                                                    float* __restrict__ nlse2, float* __restrict__ nd, int hq, int n,
-                                                   int n_pad, long long rows) {
+                                                   int n_pad, long long rows, int with_d) {
     griddep_launch_dependents();
     griddep_wait();
     constexpr int L = D / 8;  // lanes of a row, 16 bytes each
@@ -591,7 +621,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restri
     const int i = (int)(r - bh * n_pad);
     const bool in = live && i < n;
     float acc = 0.f;
-    if (in) {
+    if (in && with_d) {
         const long long b = bh / hq, h = bh - b * hq;
         const uint4 x = *reinterpret_cast<const uint4*>(o + (bh * n + i) * D + lane * 8);
         const uint4 y = *reinterpret_cast<const uint4*>(dout + b * sb + h * sh + i * sn + lane * 16);

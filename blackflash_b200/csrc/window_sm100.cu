@@ -118,6 +118,7 @@ namespace {
 struct BwdPlan {
     int nk, ns, window, sinks, n_pad, splits_s, splits_n;
     long long vec, slots, bytes;
+    bool two_sweeps;
 };
 
 BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks) {
@@ -141,6 +142,9 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     p.splits_n = norm * 2 > target * 3 ? (int)((norm + target - 1) / target) : 1;
     const long long target_s = target > norm ? target : norm;
     p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
+    // D from fp32 sums where a row sees at most a tile of keys: there the rounding of O would
+    // dominate the error of dQ and dK.
+    p.two_sweeps = p.window + p.sinks <= 128;
     p.vec = (long long)B * Hq * p.n_pad;
     p.slots = units * ((p.splits_s > 1 ? (long long)p.ns * p.splits_s : 0) +
                        (p.splits_n > 1 ? (long long)(p.nk - p.ns) * p.splits_n : 0));
@@ -210,7 +214,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
         auto kernel = d == 64 ? bfk::winb::prep_kernel<64> : bfk::winb::prep_kernel<128>;
         if ((rc = launch_error(launch_pdl(kernel, dim3(grid), 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
                                           reinterpret_cast<const char*>(dO->data), sd.s[0] * 2, sd.s[1] * 2, sd.s[2] * 2, lse,
-                                          nlse2, nd, Hq, Nq, plan.n_pad, plan.vec))) != BF_OK)
+                                          nlse2, nd, Hq, Nq, plan.n_pad, plan.vec, plan.two_sweeps ? 0 : 1))) != BF_OK)
             return rc;
     }
     const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
@@ -240,6 +244,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.q_tiles = q_tiles;
     p.splits_s = plan.splits_s;
     p.splits_n = plan.splits_n;
+    p.two_sweeps = plan.two_sweeps;
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
     p.nlse2 = nlse2;
@@ -249,6 +254,9 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.dv = reinterpret_cast<__nv_bfloat16*>(dV);
     p.part = part;
     p.timeout_ns = kTimeoutNs;
+    p.items = (int)q_items;  // first: it may leave a better D
+    rc = d == 64 ? launch_bwd<64, true>(mq, md, mk, mv, p, st) : launch_bwd<128, true>(mq, md, mk, mv, p, st);
+    if (rc != BF_OK) return rc;
     p.items = (int)kv_items;
     rc = d == 64 ? launch_bwd<64, false>(mk, mv, sq_map, sd_map, p, st) : launch_bwd<128, false>(mk, mv, sq_map, sd_map, p, st);
     if (rc != BF_OK) return rc;
@@ -262,9 +270,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     };
     if ((rc = join(part, 0, plan.ns, plan.splits_s)) != BF_OK) return rc;
     const float* rest = part + (plan.splits_s > 1 ? units * plan.ns * plan.splits_s * 2 * 128 * d : 0);
-    if ((rc = join(rest, plan.ns, plan.nk - plan.ns, plan.splits_n)) != BF_OK) return rc;
-    p.items = (int)q_items;
-    return d == 64 ? launch_bwd<64, true>(mq, md, mk, mv, p, st) : launch_bwd<128, true>(mq, md, mk, mv, p, st);
+    return join(rest, plan.ns, plan.nk - plan.ns, plan.splits_n);
 }
 
 int bf_prefix_partial(const PrefixArgs& a) {

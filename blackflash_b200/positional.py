@@ -12,54 +12,33 @@ long as the last axis is contiguous and the others step by multiples of 16 bytes
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import _require, _stream_handle
+from .ops import _require
 
-_HALF = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-_ANY = {**_HALF, torch.float32: _lib.DTYPE_F32}
+_MAX = 1 << 62
+_module = None
 
 
-def _view(t: torch.Tensor) -> _lib.View:
-    """The last three strides of [.., heads, tokens, d], and the batch's where there is one."""
-    s = t.stride()
-    return _lib.View(t.data_ptr(), (ctypes.c_longlong * 3)(s[0] if t.dim() == 4 else 0, s[-3], s[-2]))
+def _ext():
+    """The torch binding (csrc/torch_positional.cpp): it checks the arguments, allocates outputs
+    and workspaces, and calls the C ABI on the tensors' device and current stream."""
+    global _module
+    if _module is None:
+        try:
+            from . import _positional as module
+        except ImportError as e:
+            raise RuntimeError("blackflash_b200._positional is not built; build it with "
+                               "`python -m blackflash_b200.build` (needs nvcc and g++)") from e
+        _module = module
+    return _module
 
 
-def _check(name: str, t: torch.Tensor, dims: int, like: torch.Tensor | None = None, types=_HALF) -> None:
-    _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
-    _require(t.is_cuda and t.dtype in types, f"{name} must be a CUDA tensor of " +
-             ", ".join(str(x).removeprefix("torch.") for x in types))
-    _require(t.dim() == dims, f"{name} must have {dims} axes")
-    _require(t.size(-1) <= 1 or t.stride(-1) == 1, f"{name}'s last axis must be contiguous")
-    if like is not None:
-        _require(t.dtype == like.dtype and t.device == like.device, f"{name} must have Q's type and device")
-
-
-def _check_grouped(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, names=("K", "V")) -> None:
-    _check("Q", Q, 4)
-    _require(Q.size(3) in (64, 128), "BlackFlash supports d=64 and d=128")
-    for name, t in zip(names, (K, V)):
-        _check(name, t, 4, Q)
-    _require(K.shape == V.shape and K.size(0) == Q.size(0) and K.size(3) == Q.size(3),
-             f"{names[0]} and {names[1]} must have one shape, with Q's batch and d")
-    _require(K.size(1) > 0 and Q.size(1) % K.size(1) == 0, "query heads must be a multiple of KV heads")
-
-
-def _check_scale(scale: float | None, d: int) -> float:
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    _require(math.isfinite(scale) and scale > 0, "scale must be positive and finite")
-    return scale
-
-
-def _check_window(window: int, sinks: int) -> tuple[int, int]:
-    _require(window >= 1 and sinks >= 0, "need window >= 1 and sinks >= 0")
-    return min(int(window), 0x7FFFFFFF), min(int(sinks), 0x7FFFFFFF)
+def _tensors(**named) -> None:
+    for name, t in named.items():
+        _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
 
 
 # ---------------------------------------------------------------- sliding window
@@ -74,23 +53,8 @@ def window_attention_lse(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, wind
     0 and -inf. K and V must be finite in every row, those of padding too: a masked key has
     weight 0, but 0 times an infinity or NaN is NaN.
     """
-    _check_grouped(Q, K, V)
-    window, sinks = _check_window(window, sinks)
-    scale = _check_scale(scale, Q.size(3))
-    B, Hq, Nq, d = Q.shape
-    Hkv, Nkv = K.size(1), K.size(2)
-    O = torch.empty((B, Hq, Nq, d), dtype=Q.dtype, device=Q.device)
-    lse = torch.empty((B, Hq, Nq), dtype=torch.float32, device=Q.device) if want_lse else None
-    if O.numel() == 0:
-        return O, lse
-    if Nkv == 0:
-        return O.zero_(), lse.fill_(-math.inf) if want_lse else None
-    with torch.cuda.device(Q.device):
-        rc = _lib.load().blackflash_window_fwd(
-            _view(Q), _view(K), _view(V), O.data_ptr(), lse.data_ptr() if want_lse else None, B, Hq, Hkv, Nq, Nkv, d,
-            window, sinks, scale, _HALF[Q.dtype], _stream_handle(Q.device))
-    _lib.check(rc, "blackflash_window_fwd")
-    return O, lse
+    _tensors(Q=Q, K=K, V=V)
+    return _ext().window_lse(Q, K, V, min(window, _MAX), min(sinks, _MAX), scale, want_lse)
 
 
 def window_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, window: int, sinks: int = 0,
@@ -105,74 +69,18 @@ def window_attention_backward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
 
     O and lse as `window_attention_lse` returned them; dO [B, Hq, Nq, d] may be a strided
     view. dK and dV are summed over the query heads that share a KV head."""
-    _check_grouped(Q, K, V)
-    _require(Q.dtype == torch.bfloat16, "the backward supports bfloat16")
-    window, sinks = _check_window(window, sinks)
-    scale = _check_scale(scale, Q.size(3))
-    _check("O", O, 4, Q)
-    _check("dO", dO, 4, Q)
-    _require(O.shape == Q.shape and dO.shape == Q.shape and O.is_contiguous(), "O must be contiguous, O and dO of Q's shape")
-    _require(isinstance(lse, torch.Tensor) and lse.dtype == torch.float32 and lse.device == Q.device
-             and lse.is_contiguous() and lse.shape == Q.shape[:3], "lse must be a contiguous fp32 [B, Hq, Nq] tensor")
-    B, Hq, Nq, d = Q.shape
-    Hkv, Nkv = K.size(1), K.size(2)
-    dQ, dK, dV = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (Q, K, V))
-    if Q.numel() == 0 or K.numel() == 0:
-        return dQ.zero_(), dK.zero_(), dV.zero_()
-    lib = _lib.load()
-    with torch.cuda.device(Q.device):
-        nbytes = lib.blackflash_window_bwd_workspace_bytes(B, Hq, Hkv, Nq, Nkv, d, window, sinks)
-        if nbytes < 0:
-            _lib.check(_lib.BF_ERR_ARG, "blackflash_window_bwd_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
-        rc = lib.blackflash_window_bwd(
-            _view(Q), _view(K), _view(V), O.data_ptr(), _view(dO), lse.data_ptr(), dQ.data_ptr(), dK.data_ptr(),
-            dV.data_ptr(), ws.data_ptr(), nbytes, B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale, _stream_handle(Q.device))
-    _lib.check(rc, "blackflash_window_bwd")
-    return dQ, dK, dV
-
-
-class _WindowFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, Q, K, V, window, sinks, scale):
-        O, lse = window_attention_lse(Q, K, V, window, sinks, scale)
-        ctx.save_for_backward(Q, K, V, O, lse)
-        ctx.args = (window, sinks, scale)
-        return O
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dO):
-        Q, K, V, O, lse = ctx.saved_tensors
-        return (*window_attention_backward(Q, K, V, O, _rows(dO), lse, *ctx.args), None, None, None)
+    _tensors(Q=Q, K=K, V=V, O=O, dO=dO, lse=lse)
+    return _ext().window_backward(Q, K, V, O, dO, lse, min(window, _MAX), min(sinks, _MAX), scale)
 
 
 def window_attention_with_grad(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, window: int, sinks: int = 0,
                                scale: float | None = None) -> torch.Tensor:
-    """`window_attention` as a differentiable op; bf16."""
-    _require(Q.dtype == torch.bfloat16, "the backward supports bfloat16")
-    return _WindowFn.apply(Q, K, V, window, sinks, scale)
+    """`window_attention` as a differentiable op (once: no create_graph); bf16."""
+    _tensors(Q=Q, K=K, V=V)
+    return _ext().window_with_grad(Q, K, V, min(window, _MAX), min(sinks, _MAX), scale)
 
 
 # ---------------------------------------------------------------- decoding steps
-
-def _check_step(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lengths: torch.Tensor) -> None:
-    _check_grouped(Q, K, V, ("K_cache", "V_cache"))
-    _require(isinstance(lengths, torch.Tensor) and lengths.is_cuda and lengths.dtype == torch.int32
-             and lengths.device == Q.device and lengths.dim() == 1 and lengths.is_contiguous()
-             and lengths.size(0) == Q.size(0), "lengths must be a contiguous int32 [B] tensor on Q's device")
-
-
-def _step_buffers(Q: torch.Tensor, want_lse: bool, sizes: tuple):
-    """O, lse and the workspace of a decoding step."""
-    nbytes = _lib.load().blackflash_decode_workspace_bytes(*sizes)
-    if nbytes < 0:
-        _lib.check(_lib.BF_ERR_ARG, "blackflash_decode_workspace_bytes")
-    O = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
-    lse = torch.empty(Q.shape[:3], dtype=torch.float32, device=Q.device) if want_lse else None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device) if nbytes else None
-    return O, lse, ws, nbytes
-
 
 def window_decode(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor, lengths: torch.Tensor, window: int,
                   sinks: int = 0, scale: float | None = None, want_lse: bool = False):
@@ -184,22 +92,8 @@ def window_decode(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor,
     want_lse; a token that sees no key (p < 0) gets 0 and -inf. Cache rows at lengths[b]
     and after are never read and may hold anything.
     """
-    _check_step(Q, K_cache, V_cache, lengths)
-    window, sinks = _check_window(window, sinks)
-    scale = _check_scale(scale, Q.size(3))
-    B, Hq, T, d = Q.shape
-    Hkv, C = K_cache.size(1), K_cache.size(2)
-    if Q.numel() == 0 or C == 0:
-        O = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
-        return (O, torch.full((B, Hq, T), -math.inf, device=Q.device)) if want_lse else O
-    Q = Q.contiguous()
-    with torch.cuda.device(Q.device):
-        O, lse, ws, nbytes = _step_buffers(Q, want_lse, (B, Hq, Hkv, T, 0, C, d, window, sinks))
-        rc = _lib.load().blackflash_window_decode(
-            Q.data_ptr(), _view(K_cache), _view(V_cache), lengths.data_ptr(), O.data_ptr(),
-            lse.data_ptr() if want_lse else None, ws.data_ptr() if nbytes else None, nbytes, B, Hq, Hkv, T, C, d, window,
-            sinks, scale, _HALF[Q.dtype], _stream_handle(Q.device))
-    _lib.check(rc, "blackflash_window_decode")
+    _tensors(Q=Q, K_cache=K_cache, V_cache=V_cache, lengths=lengths)
+    O, lse = _ext().window_decode(Q, K_cache, V_cache, lengths, min(window, _MAX), min(sinks, _MAX), scale, want_lse)
     return (O, lse) if want_lse else O
 
 
@@ -214,26 +108,8 @@ def prefix_decode(Q: torch.Tensor, K_prefix: torch.Tensor, V_prefix: torch.Tenso
     Returns O [B, Hq, T, d], or (O, lse) with want_lse; a token that sees no key gets 0 and
     -inf. Cache rows at lengths[b] and after are never read and may hold anything.
     """
-    _check_step(Q, K_cache, V_cache, lengths)
-    for name, t in (("K_prefix", K_prefix), ("V_prefix", V_prefix)):
-        _check(name, t, 3, Q)
-    B, Hq, T, d = Q.shape
-    Hkv, C = K_cache.size(1), K_cache.size(2)
-    _require(K_prefix.shape == V_prefix.shape and K_prefix.size(0) == Hkv and K_prefix.size(2) == d,
-             "K_prefix and V_prefix must be [Hkv, P, d]")
-    scale = _check_scale(scale, d)
-    P = K_prefix.size(1)
-    if Q.numel() == 0 or P + C == 0:
-        O = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
-        return (O, torch.full((B, Hq, T), -math.inf, device=Q.device)) if want_lse else O
-    Q = Q.contiguous()
-    with torch.cuda.device(Q.device):
-        O, lse, ws, nbytes = _step_buffers(Q, want_lse, (B, Hq, Hkv, T, P, C, d, 0x7FFFFFFF, 0))
-        rc = _lib.load().blackflash_prefix_decode(
-            Q.data_ptr(), _view(K_prefix), _view(V_prefix), _view(K_cache), _view(V_cache), lengths.data_ptr(),
-            O.data_ptr(), lse.data_ptr() if want_lse else None, ws.data_ptr() if nbytes else None, nbytes, B, Hq, Hkv, T, P,
-            C, d, scale, _HALF[Q.dtype], _stream_handle(Q.device))
-    _lib.check(rc, "blackflash_prefix_decode")
+    _tensors(Q=Q, K_prefix=K_prefix, V_prefix=V_prefix, K_cache=K_cache, V_cache=V_cache, lengths=lengths)
+    O, lse = _ext().prefix_decode(Q, K_prefix, V_prefix, K_cache, V_cache, lengths, scale, want_lse)
     return (O, lse) if want_lse else O
 
 
@@ -290,54 +166,13 @@ def rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, freqs: tor
     rotated part are copied. inverse turns the other way (the gradient's map). bf16, fp16 or
     fp32, any even d up to 1024; returns contiguous (Q', K').
     """
-    _check("Q", Q, 4, types=_ANY)
-    _check("K", K, 4, Q, types=_ANY)
-    B, Hq, N, d = Q.shape
-    _require(K.size(0) == B and K.size(2) == N and K.size(3) == d, "K must have Q's batch, tokens and d")
-    for name, t in (("positions", positions), ("freqs", freqs)):
-        _require(isinstance(t, torch.Tensor) and t.device == Q.device and t.is_contiguous(),
-                 f"{name} must be a contiguous tensor on Q's device")
-    _require(positions.dtype in (torch.int32, torch.int64) and positions.shape in ((N,), (B, N)),
-             "positions must be int32 or int64, [N] or [B, N]")
-    _require(freqs.dtype == torch.float64 and freqs.dim() == 1, "freqs must be fp64 [rotary_dim / 2]")
-    rot = 2 * freqs.numel()
-    _require(d % 2 == 0 and d <= 1024 and 2 <= rot <= d, "need an even d <= 1024 and 1 to d / 2 frequencies")
-    _require(math.isfinite(amplitude), "amplitude must be finite")
-    Qo = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
-    Ko = torch.empty(K.shape, dtype=Q.dtype, device=Q.device)
-    if Qo.numel() + Ko.numel() == 0:
-        return Qo, Ko
-    with torch.cuda.device(Q.device):
-        rc = _lib.load().blackflash_rotary(
-            _view(Q), _view(K), Qo.data_ptr(), Ko.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64,
-            positions.dim() == 2, freqs.data_ptr(), B, Hq, K.size(1), N, d, rot, bool(interleaved), float(amplitude),
-            bool(inverse), _ANY[Q.dtype], _stream_handle(Q.device))
-    _lib.check(rc, "blackflash_rotary")
-    return Qo, Ko
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, Q, K, positions, freqs, interleaved, amplitude):
-        ctx.save_for_backward(positions, freqs)
-        ctx.args = (interleaved, amplitude)
-        return rotary(Q, K, positions, freqs, interleaved, amplitude)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dQ, dK):
-        # The map is linear, so its gradient is its transpose: the same turn backwards.
-        positions, freqs = ctx.saved_tensors
-        dQ, dK = rotary(_rows(dQ), _rows(dK), positions, freqs, *ctx.args, inverse=True)
-        return dQ, dK, None, None, None, None
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A gradient as the kernels read it: its rows contiguous, and not broadcast."""
-    return t if t.stride(-1) == 1 and 0 not in t.stride() else t.contiguous()
+    _tensors(Q=Q, K=K, positions=positions, freqs=freqs)
+    return _ext().rotary(Q, K, positions, freqs, interleaved, amplitude, inverse)
 
 
 def rotary_with_grad(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
                      interleaved: bool = False, amplitude: float = 1.0):
-    """`rotary` as a differentiable op; gradients for Q and K, not for the frequencies."""
-    return _RotaryFn.apply(Q, K, positions, freqs, interleaved, amplitude)
+    """`rotary` as a differentiable op (once: no create_graph); gradients for Q and K, not for
+    the frequencies."""
+    _tensors(Q=Q, K=K, positions=positions, freqs=freqs)
+    return _ext().rotary_with_grad(Q, K, positions, freqs, interleaved, amplitude)

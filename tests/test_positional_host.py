@@ -125,6 +125,8 @@ def test_python_checks():
     z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t)  # noqa: E731
     q, n = z(1, 2, 4, 64), torch.zeros(1, dtype=torch.int32)
     f = torch.zeros(32, dtype=torch.float64)
+    from blackflash_b200.build import build_torch_ext
+    build_torch_ext()
     for call in (lambda: bf.window_attention(q, q, q, 4), lambda: bf.window_attention(q.float(), q, q, 4),
                  lambda: bf.window_attention_lse(None, q, q, 4), lambda: bf.window_decode(q, q, q, n, 4),
                  lambda: bf.prefix_decode(q, q[0], q[0], q, q, n), lambda: bf.rotary(q, q, n, f)):
