@@ -422,10 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int part = 0; part < D / 64; ++part) {
                 uint32_t o[32];
-                if (steps > 0) {
-                    tmem_ld16x32bx2_x32<D / 2>(tO + 32 * part, o);
-                    tmem_wait_ld();
-                }
+                tmem_ld16x32bx2_x32<D / 2>(tO + 32 * part, o);  // without steps: anything, and not used
+                tmem_wait_ld();
                 if (empty) {
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] = 0u;
