@@ -13,7 +13,7 @@
 // the result does not depend on the order of the blocks.
 //
 // Both passes are one kernel. A work item keeps two stationary 128-row tiles X0, X1 and
-// streams pairs of NT-row tiles Y0, Y1 past them:
+// streams pairs of 64-row tiles Y0, Y1 past them:
 //                    X0  X1   Y0  Y1    S = X0 Y0^T   dP = X1 Y1^T   accumulators
 //   dK/dV (kDQ=0)    K   V    Q   dO    (S^T)         (dP^T)         dV += P^T Y1, dK += dS^T Y0
 //   dQ    (kDQ=1)    Q   dO   K   V                                  dQ += dS Y0
@@ -22,41 +22,48 @@
 // is then a large part (one key: dP - D is 0). So with few keys (two_sweeps) the dQ pass
 // walks its KV tiles twice: first it sums P dP and P in fp32, D = sum P dP / sum P, which it
 // also leaves in the array for the dK/dV pass; then it accumulates.
-// Roles: eight elementwise warps (two threads per row), a TMA producer, an issuer of S and
-// dP, an issuer of the accumulations; persistent blocks, so an item's tail overlaps the next
-// one's first products. S has two buffers: S of step n + 1 is computed while the elementwise
-// warps are at step n. P and dS go back to TMEM as bf16, over the S buffer they came from,
-// and are the A operands of the accumulations; neither leaves the SM.
-// TMEM (512 columns):  dK/dV d=64: S 2x128, dP 128, dV 64, dK 64
-//                      dK/dV d=128: NT = 64 queries: S 2x64, dP 2x64, dV 128, dK 128
-//                      dQ: S 2x128, dP 128, dQ 64 / 128
+// Roles: two groups of eight elementwise warps (two threads per row), which take the steps in
+// turn: a step is a chain of TMEM loads, exponentials and stores that one group alone leaves
+// mostly waiting, so the other one's chain runs under it; a TMA producer; one issuer each of S,
+// dP and the accumulations (an MMA takes about 60 cycles to issue here, so one warp for S and
+// dP was itself the limit). Blocks are persistent, so an item's tail overlaps the next one's
+// first products.
+// TMEM (512 columns): four 64-column buffers, the accumulators from 256 on. Everything of a
+// step happens in one buffer: S is computed there and loaded; dP is computed over it while the
+// exponentials run; P and dS, as bf16 the A operands of the accumulations, go over dP. With two
+// buffers a group, no step waits for the accumulations of the step before (with S and dP
+// buffers apart, one each a group, it did: 1970 cycles a step against the tensor core's 1020).
+// P stays fp32 until it is multiplied by dP - D, so that dS is rounded once. 64-row streamed
+// tiles leave that room, and 32 columns a thread fit the 104 registers that sixteen
+// elementwise warps can have; the price is that S and dP, 64 wide, are bound by reading their
+// stationary operand from shared memory (48 cycles an MMA instead of 32).
 namespace winb {
 
 using win::kTmemCols;
 
-constexpr int kThreads = 12 * 32;
-constexpr int kEwWarps = 8;
-constexpr int kProdWarp = 8;
-constexpr int kFrontWarp = 9;  // issues S and dP; owns the TMEM allocation
-constexpr int kAccWarp = 10;   // issues the accumulations; warp 11 completes the warpgroup
-constexpr int kEwRegs = 216, kOtherRegs = 64;  // launch budget 384 x 168
-static_assert(kEwWarps * 32 * kEwRegs + 128 * kOtherRegs <= kThreads * 168, "register split exceeds the launch budget");
+constexpr int kThreads = 20 * 32;
+constexpr int kGroupWarps = 8, kEwWarps = 2 * kGroupWarps;
+constexpr int kProdWarp = 16;
+constexpr int kFrontWarp = 17;  // issues S (and owns the TMEM allocation); 18 dP; 19 the accumulations
+constexpr int kEwRegs = 104, kOtherRegs = 64;  // launch budget 640 x 96
+static_assert(kEwWarps * 32 * kEwRegs + 128 * kOtherRegs <= kThreads * 96, "register split exceeds the launch budget");
+constexpr int NT = 64;       // rows of a streamed tile
+constexpr int NC = NT / 2;   // of them (S columns) a thread's
+constexpr int kBufs = 4;     // S / dP / P, dS buffers; step n uses buffer n % 4
+constexpr int kColAcc = kBufs * NT;
 
 template <int D, bool kDQ>
 struct Cfg {
-    static constexpr int NT = !kDQ && D == 128 ? 64 : 128;  // rows of a streamed tile
     static constexpr int kChunks = D / 64;
     static constexpr int kXChunk = 128 * 128, kXTile = kChunks * kXChunk;
     static constexpr int kYChunk = NT * 128, kYTile = kChunks * kYChunk;
-    static constexpr int kStages = kDQ && D == 128 ? 2 : 4;
+    static constexpr int kStages = D == 128 ? 4 : 6;
     static constexpr int kVec = kDQ ? 0 : 2 * NT * 4;  // -lse2 and -D of the streamed queries
     static constexpr int kOffX = 0;
     static constexpr int kOffY = kOffX + 2 * kXTile;              // [kStages][Y0, Y1]
     static constexpr int kOffVec = kOffY + kStages * 2 * kYTile;  // [kStages]
-    static constexpr int kOffBar = kOffVec + kStages * kVec;
-    static constexpr int kDpBufs = NT == 64 ? 2 : 1;
-    static constexpr int kColDP = 2 * NT;
-    static constexpr int kColAcc = kColDP + kDpBufs * NT;
+    static constexpr int kOffSum = kOffVec + kStages * kVec;      // dQ: [2][2 groups][128] {sum P, sum P dP}
+    static constexpr int kOffBar = kOffSum + (kDQ ? 4096 : 0);
     static constexpr int kAccs = kDQ ? 1 : 2;
     static_assert(kColAcc + kAccs * D <= kTmemCols, "TMEM columns");
 };
@@ -65,10 +72,12 @@ template <int D, bool kDQ>
 struct Bars {
     uint64_t x_full, x_empty;
     uint64_t y_full[Cfg<D, kDQ>::kStages], y_empty[Cfg<D, kDQ>::kStages];
-    uint64_t s_full[2], s_free[2], p_ready[2];
-    uint64_t dp_full[2], dp_free[2];
+    uint64_t s_full[kBufs], s_read[kBufs];    // S computed; loaded by the group
+    uint64_t dp_full[kBufs], p_ready[kBufs];  // dP computed; P, dS written
+    uint64_t buf_free[kBufs];                 // the accumulations have read P, dS
     uint64_t acc_full, acc_free;
-    uint64_t drain[2];
+    uint64_t sums;  // dQ, two sweeps: every warp's sums are in shared memory
+    uint64_t drain[3];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -93,6 +102,7 @@ enum : unsigned {
     kSiteEwS = 0x830,
     kSiteEwDP = 0x831,
     kSiteEwAcc = 0x832,
+    kSiteEwSums = 0x833,
 };
 
 struct Params {
@@ -122,7 +132,6 @@ struct Item {
 };
 
 // First query tile and number of query tiles (NT rows) that see KV tile j.
-template <int NT>
 __device__ __forceinline__ void queries_of(const Params& p, int j, int& i0, int& ni) {
     const int off = p.n_kv - p.n_q;
     const int last_key = min(j * 128 + 127, p.n_kv - 1);
@@ -144,9 +153,9 @@ __device__ __forceinline__ void decode(const Params& p, int item, Item& it) {
         it.kvh = it.head / p.group;
         const int off = p.n_kv - p.n_q;
         const int p_first = it.tile * 128 + off, p_last = min(it.tile * 128 + 128, p.n_q) - 1 + off;
-        const int lo = max(0, p_first - p.window + 1) >> 7;
-        const int hi = p_last >= 0 ? (p_last >> 7) + 1 : 0;
-        it.n_sink = min(p.ns, lo);
+        const int lo = max(0, p_first - p.window + 1) / NT;
+        const int hi = p_last >= 0 ? p_last / NT + 1 : 0;
+        it.n_sink = min((p.sinks + NT - 1) / NT, lo);
         it.skip = lo - it.n_sink;
         it.steps = hi > 0 ? hi - it.skip : 0;
         it.slot = -1;
@@ -172,7 +181,7 @@ __device__ __forceinline__ void decode(const Params& p, int item, Item& it) {
             const long long base = p.splits_s > 1 ? (long long)units * sink_items : 0;
             it.slot = splits > 1 ? base + ((long long)unit * (p.nk - p.ns) + it.tile - p.ns) * splits + part : -1;
         }
-        queries_of<Cfg<D, kDQ>::NT>(p, it.tile, it.i0, it.ni);
+        queries_of(p, it.tile, it.i0, it.ni);
         const long long len = (long long)it.ni * p.group;
         it.s0 = (int)(len * part / splits);
         it.steps = (int)(len * (part + 1) / splits) - it.s0;
@@ -184,31 +193,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     window_bwd_kernel(const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1,
                       const __grid_constant__ CUtensorMap tmY0, const __grid_constant__ CUtensorMap tmY1, const Params p) {
     using C = Cfg<D, kDQ>;
-    constexpr int NT = C::NT;
-    constexpr int NC = NT / 2;  // streamed rows (S columns) of a thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     Bars<D, kDQ>* bars = reinterpret_cast<Bars<D, kDQ>*>(smem + C::kOffBar);
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // known to be uniform
     const int lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(smem_addr(&bars->x_full), 1);
-        mbar_init(smem_addr(&bars->x_empty), 1);
+        mbar_init(smem_addr(&bars->x_empty), 2);  // S and dP each
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(smem_addr(&bars->y_full[s]), 1);
             mbar_init(smem_addr(&bars->y_empty[s]), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kBufs; ++b) {
             mbar_init(smem_addr(&bars->s_full[b]), 1);
-            mbar_init(smem_addr(&bars->s_free[b]), 1);
-            mbar_init(smem_addr(&bars->p_ready[b]), kEwWarps);  // one arrival per elementwise warp
+            mbar_init(smem_addr(&bars->s_read[b]), kGroupWarps);  // one arrival per elementwise warp of the group
             mbar_init(smem_addr(&bars->dp_full[b]), 1);
-            mbar_init(smem_addr(&bars->dp_free[b]), kEwWarps);
-            mbar_init(smem_addr(&bars->drain[b]), 1);
+            mbar_init(smem_addr(&bars->p_ready[b]), kGroupWarps);
+            mbar_init(smem_addr(&bars->buf_free[b]), 1);
         }
+        for (int r = 0; r < 3; ++r) mbar_init(smem_addr(&bars->drain[r]), 1);
         mbar_init(smem_addr(&bars->acc_full), 1);
         mbar_init(smem_addr(&bars->acc_free), kEwWarps);
+        mbar_init(smem_addr(&bars->sums), kEwWarps);
         bars->abort_flag = 0;
         fence_barrier_init();
     }
@@ -237,77 +245,79 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < kEwWarps) {
         // ------------------------------------------------------------ elementwise
+        const int grp = warp >> 3;  // takes the steps n with n % 2 == grp
         const int quarter = warp & 3;
-        const int sub = warp >> 2;
+        const int sub = (warp >> 2) & 1;
         const int h = lane >> 4;                                // S columns NC h .. NC h + NC - 1
         const int row = quarter * 32 + sub * 16 + (lane & 15);  // row of the tile == TMEM lane
         const uint32_t tl = tmem + ((uint32_t)(quarter * 32 + sub * 16) << 16);
         const int off = p.n_kv - p.n_q;
         const uint64_t sl2_2 = f2_pack(p.scale_log2, p.scale_log2);
-        uint32_t n = 0;  // steps so far
-        int n_it = 0;    // items with steps so far
+        uint32_t n0 = 0;  // steps of the items before
+        int n_it = 0;     // items with steps so far
         bool ok = true;
-        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-            Item it;
-            decode<D, kDQ>(p, item, it);
-            const int xrow = it.tile * 128 + row;
-            // dQ: the row's -lse2 and -D (padded rows have entries).
-            const int lead = kDQ && p.two_sweeps ? it.steps : 0;  // steps of the first sweep
-            const size_t at = kDQ ? ((size_t)it.b * p.hq + it.head) * p.n_pad + xrow : 0;
-            uint64_t nl2 = 0, nd2 = 0;
-            float sum_p = 0.f, sum_pdp = 0.f;
+        // dQ: the next item is decoded, and its rows' -lse2 and -D requested, before the current
+        // one's gradients are waited for (dK/dV has more steps an item and no registers for it).
+        Item next;
+        float next_l = 0.f, next_d = 0.f;  // dQ (padded rows have entries)
+        auto fetch = [&](int item) {
+            if (item >= p.items) return;
+            decode<D, kDQ>(p, item, next);
             if constexpr (kDQ) {
-                const float a = p.nlse2[at], b = lead ? 0.f : p.nd[at];
-                nl2 = f2_pack(a, a);
-                nd2 = f2_pack(b, b);
+                const size_t at = ((size_t)next.b * p.hq + next.head) * p.n_pad + next.tile * 128 + row;
+                next_l = p.nlse2[at];
+                next_d = p.two_sweeps ? 0.f : p.nd[at];
             }
-            for (int s_all = 0; s_all < lead + it.steps; ++s_all, ++n) {
-                const bool measure = kDQ && s_all < lead;
-                const int s_i = measure || !kDQ ? s_all : s_all - lead;
-                if (kDQ && lead && s_all == lead) {
-                    // The two halves of the row; a row that sees nothing has D = 0.
-                    sum_p += __shfl_xor_sync(0xffffffffu, sum_p, 16);
-                    sum_pdp += __shfl_xor_sync(0xffffffffu, sum_pdp, 16);
-                    const float b = sum_p != 0.f ? -sum_pdp / sum_p : 0.f;
-                    nd2 = f2_pack(b, b);
-                    if (h == 0) p.nd[at] = b;
-                }
-                const int buf = n & 1;
-                const uint32_t tS = tl + (uint32_t)(buf * NT);
+        };
+        if constexpr (kDQ) fetch(blockIdx.x);
+        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+            if constexpr (!kDQ) fetch(item);
+            const Item it = next;
+            const int xrow = it.tile * 128 + row;
+            const int lead = kDQ && p.two_sweeps ? it.steps : 0;  // steps of the first sweep
+            uint64_t nl2 = f2_pack(next_l, next_l), nd2 = f2_pack(next_d, next_d);
+            int q_tile = 0;  // dK/dV: the next step's query tile, from i0 on
+            // One step; in the first sweep (measure) it only adds up P and P dP.
+            float sum_p = 0.f, sum_pdp = 0.f;
+            auto step = [&](int s_i, uint32_t n, bool measure) -> bool {
+                const uint32_t buf = n & (kBufs - 1), par = (n / kBufs) & 1u;
+                const uint32_t tB = tl + buf * NT;
                 // Visible: column c with c < last and (c >= first or c < snk).
                 int first, last, snk;
                 if constexpr (kDQ) {
-                    const int c0 = (s_i < it.n_sink ? s_i : s_i + it.skip) * 128 + h * NC;
+                    const int c0 = (s_i < it.n_sink ? s_i : s_i + it.skip) * NT + h * NC;
                     last = xrow + off + 1 - c0;
                     first = xrow + off + 1 - p.window - c0;
                     snk = p.sinks - c0;
                 } else {
-                    const int q0 = (it.i0 + (it.s0 + s_i) % it.ni) * NT + h * NC;
+                    const int q0 = (it.i0 + q_tile) * NT + h * NC;
                     first = xrow - off - q0;
                     last = xrow < p.sinks ? NC : first + p.window;
                     snk = 0;
                 }
-                if (!(ok = warp_wait(smem_addr(&bars->s_full[buf]), (n >> 1) & 1u, ctl, kSiteEwS))) break;
+                if (!warp_wait(smem_addr(&bars->s_full[buf]), par, ctl, kSiteEwS)) return false;
                 tc_fence_after();
                 float pr[NC];
                 {
-                    uint32_t s[NC / 32][32];
-#pragma unroll
-                    for (int i = 0; i < NC / 32; ++i) tmem_ld16x32bx2_x32<NC>(tS + 32 * i, s[i]);
+                    uint32_t s[NC];
+                    tmem_ld16x32bx2_x32<NC>(tB, s);
                     tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&bars->s_read[buf]));  // dP may be computed over it
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) pr[c] = __uint_as_float(s[c >> 5][c & 31]);
+                    for (int c = 0; c < NC; ++c) pr[c] = __uint_as_float(s[c]);
                 }
+                const float* vec = reinterpret_cast<const float*>(smem + C::kOffVec + (n % C::kStages) * C::kVec) + h * NC;
                 if constexpr (!kDQ) {
                     // The vectors came with Y; seen here too, their copy is visible to this warp.
-                    if (!(ok = warp_wait(smem_addr(&bars->y_full[n % C::kStages]), (n / C::kStages) & 1u, ctl, kSiteEwS))) break;
+                    if (!warp_wait(smem_addr(&bars->y_full[n % C::kStages]), (n / C::kStages) & 1u, ctl, kSiteEwS)) return false;
                 }
                 if (last < NC || (first > 0 && snk < NC)) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
                         if (c >= last || (c < first && c >= snk)) pr[c] = -INFINITY;
                 }
-                const float* vec = reinterpret_cast<const float*>(smem + C::kOffVec + (n % C::kStages) * C::kVec) + h * NC;
 #pragma unroll
                 for (int c = 0; c < NC; c += 4) {
                     uint64_t a = nl2, b = nl2;
@@ -324,63 +334,82 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pr[c + 2] = fast_exp2(x2);
                     pr[c + 3] = fast_exp2(x3);
                 }
-                if constexpr (!kDQ) {
-                    // P^T as bf16 over S's first half (this thread: words NC h / 2 ..).
-#pragma unroll
-                    for (int i = 0; i < NC / 32; ++i) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) pk[c] = pack_bf16x2(pr[32 * i + 2 * c], pr[32 * i + 2 * c + 1]);
-                        tmem_st16x32bx2_x16<NC / 2>(tS + 16 * i, pk);
-                    }
-                }
                 // dS = P (dP - D)
-                const int db = C::kDpBufs == 2 ? buf : 0;
-                const uint32_t dpar = (C::kDpBufs == 2 ? n >> 1 : n) & 1u;
-                if (!(ok = warp_wait(smem_addr(&bars->dp_full[db]), dpar, ctl, kSiteEwDP))) break;
+                if (!warp_wait(smem_addr(&bars->dp_full[buf]), par, ctl, kSiteEwDP)) return false;
                 tc_fence_after();
-                uint32_t dsk[NC / 2];
+                uint32_t dp[NC];
+                tmem_ld16x32bx2_x32<NC>(tB, dp);
+                tmem_wait_ld();
+                // P^T over the first half of the buffer (this thread: words NC h / 2 ..), dS^T over
+                // the second; dQ needs dS alone.
+                uint32_t pk[NC / 2];
+                if constexpr (!kDQ) {
 #pragma unroll
-                for (int i = 0; i < NC / 32; ++i) {
-                    uint32_t dp[32];
-                    tmem_ld16x32bx2_x32<NC>(tl + C::kColDP + db * NT + 32 * i, dp);
-                    tmem_wait_ld();
-                    if (i == NC / 32 - 1) {  // dP is in registers: the next one may be computed
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_addr(&bars->dp_free[db]));
-                    }
+                    for (int c = 0; c < NC / 2; ++c) pk[c] = pack_bf16x2(pr[2 * c], pr[2 * c + 1]);
+                    tmem_st16x32bx2_x16<NC / 2>(tB, pk);
+                }
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        uint64_t a = nd2, b = nd2;
-                        if constexpr (!kDQ) {
-                            const float4 v = *reinterpret_cast<const float4*>(vec + NT + 32 * i + c);
-                            a = f2_pack(v.x, v.y);
-                            b = f2_pack(v.z, v.w);
-                        }
-                        float x0, x1, x2, x3;
-                        f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), a), x0, x1);
-                        f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c + 2]), __uint_as_float(dp[c + 3])), b), x2, x3);
-                        if (kDQ && measure) {  // D is 0 so far: x is dP
-                            const float* q = pr + 32 * i + c;
-                            sum_p += (q[0] + q[1]) + (q[2] + q[3]);
-                            sum_pdp += (q[0] * x0 + q[1] * x1) + (q[2] * x2 + q[3] * x3);
-                        }
-                        dsk[16 * i + c / 2] = pack_bf16x2(pr[32 * i + c] * x0, pr[32 * i + c + 1] * x1);
-                        dsk[16 * i + c / 2 + 1] = pack_bf16x2(pr[32 * i + c + 2] * x2, pr[32 * i + c + 3] * x3);
+                for (int c = 0; c < NC; c += 4) {
+                    uint64_t a = nd2, b = nd2;
+                    if constexpr (!kDQ) {
+                        const float4 v = *reinterpret_cast<const float4*>(vec + NT + c);
+                        a = f2_pack(v.x, v.y);
+                        b = f2_pack(v.z, v.w);
                     }
+                    float x0, x1, x2, x3;
+                    f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), a), x0, x1);
+                    f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c + 2]), __uint_as_float(dp[c + 3])), b), x2, x3);
+                    x0 *= pr[c];
+                    x1 *= pr[c + 1];
+                    x2 *= pr[c + 2];
+                    x3 *= pr[c + 3];
+                    if (kDQ && measure) {  // D is 0 so far: x is P dP
+                        sum_p += (pr[c] + pr[c + 1]) + (pr[c + 2] + pr[c + 3]);
+                        sum_pdp += (x0 + x1) + (x2 + x3);
+                    }
+                    pk[c / 2] = pack_bf16x2(x0, x1);
+                    pk[c / 2 + 1] = pack_bf16x2(x2, x3);
                 }
                 if (!measure) {
-#pragma unroll
-                    for (int i = 0; i < NC / 32; ++i)
-                        tmem_st16x32bx2_x16<NC / 2>(tS + (kDQ ? 0 : NT / 2) + 16 * i, dsk + 16 * i);
+                    tmem_st16x32bx2_x16<NC / 2>(tB + (kDQ ? 0 : NT / 2), pk);
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&bars->p_ready[buf]));
+                return true;
+            };
+            int s_all = (int)((n0 ^ (uint32_t)grp) & 1u);  // this group's first step of the item
+            if constexpr (kDQ) {
+                for (; s_all < lead && ok; s_all += 2) ok = step(s_all, n0 + s_all, true);
+                if (!ok) break;
+                if (lead > 0) {
+                    // D from the four sums of the row: two column halves, two groups.
+                    sum_p += __shfl_xor_sync(0xffffffffu, sum_p, 16);
+                    sum_pdp += __shfl_xor_sync(0xffffffffu, sum_pdp, 16);
+                    float2* sums = reinterpret_cast<float2*>(smem + C::kOffSum) + (n_it & 1) * 256;
+                    if (h == 0) sums[grp * 128 + row] = make_float2(sum_p, sum_pdp);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&bars->sums));
+                    if (!(ok = warp_wait(smem_addr(&bars->sums), (uint32_t)n_it & 1u, ctl, kSiteEwSums))) break;
+                    const float2 x = sums[row], y = sums[128 + row];
+                    const float tp = x.x + y.x, tpdp = x.y + y.y;
+                    const float b = tp != 0.f ? -tpdp / tp : 0.f;  // a row that sees nothing has D = 0
+                    nd2 = f2_pack(b, b);
+                    if (grp == 0 && h == 0) p.nd[((size_t)it.b * p.hq + it.head) * p.n_pad + xrow] = b;
+                }
+            }
+            if constexpr (!kDQ) q_tile = it.ni > 0 ? (it.s0 + s_all) % it.ni : 0;
+            for (; s_all < lead + it.steps && ok; s_all += 2) {
+                ok = step(s_all - lead, n0 + s_all, false);
+                if constexpr (!kDQ) {
+                    q_tile += 2;
+                    while (q_tile >= it.ni) q_tile -= it.ni;  // into the next head's tiles
+                }
             }
             if (!ok) break;
+            n0 += (uint32_t)(lead + it.steps);
+            if constexpr (kDQ) fetch(item + gridDim.x);
 
             // ---------------------------------------------------- the item's gradients
             const bool any = it.steps > 0;
@@ -389,14 +418,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++n_it;
                 tc_fence_after();
             }
+            // 32-column pieces of a thread: the groups take them in turn (dK/dV: 0 dV, 1 dK).
+            constexpr int kPieces = C::kAccs * (D / 64);
 #pragma unroll 1
-            for (int i = 0; i < C::kAccs * (D / 64); ++i) {
-                const int which = i / (D / 64), part = i % (D / 64);  // dK/dV: 0 dV, 1 dK
+            for (int i = grp ? (kPieces + 1) / 2 : 0; i < (grp ? kPieces : (kPieces + 1) / 2); ++i) {
+                const int which = i / (D / 64), part = i % (D / 64);
                 uint32_t o[32];
-                if (any) {
-                    tmem_ld16x32bx2_x32<D / 2>(tl + C::kColAcc + which * D + 32 * part, o);
-                    tmem_wait_ld();
-                } else {
+                tmem_ld16x32bx2_x32<D / 2>(tl + kColAcc + which * D + 32 * part, o);
+                tmem_wait_ld();
+                if (!any) {
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] = 0u;
                 }
@@ -452,6 +482,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++n_it;
             __syncwarp();
             const int lead = kDQ && p.two_sweeps ? it.steps : 0;
+            int g = 0, i = 0;  // dK/dV: head of the group and query tile of the next step
+            if constexpr (!kDQ) {
+                g = it.s0 / it.ni;
+                i = it.s0 - g * it.ni;
+            }
             for (int s_all = 0; s_all < lead + it.steps; ++s_all, ++n) {
                 const int s_i = s_all < lead ? s_all : s_all - lead;
                 const uint32_t f = smem_addr(&bars->y_full[st]);
@@ -462,9 +497,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         yrow = (s_i < it.n_sink ? s_i : s_i + it.skip) * NT;
                         head = it.kvh;
                     } else {
-                        const int s = it.s0 + s_i;
-                        yrow = (it.i0 + s % it.ni) * NT;
-                        head = it.kvh * p.group + s / it.ni;
+                        yrow = (it.i0 + i) * NT;
+                        head = it.kvh * p.group + g;
                     }
                     mbar_arrive_expect_tx(f, 2 * C::kYTile + C::kVec);
                     const uint32_t y = y0 + (uint32_t)(st * 2 * C::kYTile);
@@ -479,6 +513,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 __syncwarp();
+                if (!kDQ && ++i == it.ni) {
+                    i = 0;
+                    ++g;
+                }
                 if (++st == C::kStages) {
                     st = 0;
                     par ^= 1u;
@@ -495,90 +533,80 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_wait(smem_addr(&bars->y_full[(n - s) % C::kStages]), (uint32_t)((n - s) / C::kStages) & 1u, drain, 0);
         }
         __syncwarp();
-    } else if (warp == kFrontWarp || warp == kAccWarp) {
+    } else if (warp >= kFrontWarp) {
         // ------------------------------------------------------------ MMA issuers
         constexpr uint32_t kIdescS = idesc_bf16_f32(128, NT, 0);  // K-major x K-major
-        constexpr uint32_t kIdescG = idesc_bf16_f32(128, 64, 1);  // TMEM x MN-major 64-column chunk
-        const bool leader = elect_one();
+        constexpr uint32_t kIdescG = idesc_bf16_f32(128, D, 1);   // TMEM x MN-major, D wide
+        const uint32_t on = elect_one() ? 1u : 0u;
+        // MN-major operands step by a chunk from 64 columns to the next 64 (leading dimension).
         const uint64_t desc_base = smem_desc_sw128(smem_addr(smem), 16, 1024);
         const uint32_t desc_hi = (uint32_t)(desc_base >> 32);
         const uint32_t lo0 = (uint32_t)desc_base;
-        const uint32_t x_lo = lo0 + (C::kOffX >> 4), y_lo0 = lo0 + (C::kOffY >> 4);
-        const bool front = warp == kFrontWarp;
-        uint32_t n = 0;
-        int n_it = 0, st = 0;
-        uint32_t par = 0;
+        const uint32_t lo0_mn = (uint32_t)smem_desc_sw128(smem_addr(smem), C::kYChunk, 1024);
+        const int role = warp - kFrontWarp;  // 0 S, 1 dP, 2 accumulations
+        uint32_t n = 0, st = 0, par = 0;     // step, its stage and the stage's parity
+        int n_it = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
             Item it;
             decode<D, kDQ>(p, item, it);
             if (it.steps == 0) continue;
-            if (front) {
+            const int lead = kDQ && p.two_sweeps ? it.steps : 0, last = lead + it.steps - 1;
+            if (role < 2) {
                 if (!(ok = warp_wait(smem_addr(&bars->x_full), (uint32_t)n_it & 1u, ctl, kSiteFrontX))) break;
                 tc_fence_after();
             }
-            const int lead = kDQ && p.two_sweeps ? it.steps : 0, last = lead + it.steps - 1;
-            for (int s_i = 0; s_i <= last; ++s_i, ++n) {
-                const int buf = n & 1;
-                const uint32_t y_lo = y_lo0 + (uint32_t)(st * 2 * C::kYTile >> 4);
-                const uint32_t tS = tmem + (uint32_t)(buf * NT);
-                if (front) {
+            for (int s = 0; s <= last; ++s, ++n) {
+                const uint32_t buf = n & (kBufs - 1), use = n / kBufs;
+                const uint32_t y = lo0 + (C::kOffY >> 4) + st * (2 * C::kYTile >> 4);
+                if (role == 0) {
+                    // S of the step, once the accumulations of four steps before have read the buffer.
                     if (!(ok = warp_wait(smem_addr(&bars->y_full[st]), par, ctl, kSiteFrontY))) break;
-                    if (n >= 2 && !(ok = warp_wait(smem_addr(&bars->s_free[buf]), ((n >> 1) - 1) & 1u, ctl, kSiteFrontS))) break;
+                    if (use > 0 && !(ok = warp_wait(smem_addr(&bars->buf_free[buf]), (use - 1) & 1u, ctl, kSiteFrontS))) break;
                     tc_fence_after();
-                    if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            umma_ss_lo(tS, x_lo + (uint32_t)(kk >> 2) * (C::kXChunk >> 4) + (uint32_t)(kk & 3) * 2,
-                                       y_lo + (uint32_t)(kk >> 2) * (C::kYChunk >> 4) + (uint32_t)(kk & 3) * 2, desc_hi,
-                                       kIdescS, kk > 0);
-                        umma_commit(smem_addr(&bars->s_full[buf]));
-                    }
-                    __syncwarp();
-                    const int db = C::kDpBufs == 2 ? buf : 0;
-                    const uint32_t uses = C::kDpBufs == 2 ? n >> 1 : n;  // earlier uses of this dP buffer
-                    if (uses > 0 && !(ok = warp_wait(smem_addr(&bars->dp_free[db]), (uses - 1) & 1u, ctl, kSiteFrontDP))) break;
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        umma_ss_on(on, tmem + buf * NT, lo0 + (C::kOffX >> 4) + (kk >> 2) * (C::kXChunk >> 4) + (kk & 3) * 2,
+                                   y + (kk >> 2) * (C::kYChunk >> 4) + (kk & 3) * 2, desc_hi, kIdescS, kk > 0);
+                    umma_commit_on(on, smem_addr(&bars->s_full[buf]));
+                    if (s == last) umma_commit_on(on, smem_addr(&bars->x_empty));
+                } else if (role == 1) {
+                    // dP over S, once the group has loaded S.
+                    if (!(ok = warp_wait(smem_addr(&bars->y_full[st]), par, ctl, kSiteFrontY))) break;
+                    if (!(ok = warp_wait(smem_addr(&bars->s_read[buf]), use & 1u, ctl, kSiteFrontDP))) break;
                     tc_fence_after();
-                    if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            umma_ss_lo(tmem + C::kColDP + db * NT,
-                                       x_lo + (C::kXTile >> 4) + (uint32_t)(kk >> 2) * (C::kXChunk >> 4) + (uint32_t)(kk & 3) * 2,
-                                       y_lo + (C::kYTile >> 4) + (uint32_t)(kk >> 2) * (C::kYChunk >> 4) + (uint32_t)(kk & 3) * 2,
-                                       desc_hi, kIdescS, kk > 0);
-                        umma_commit(smem_addr(&bars->dp_full[db]));
-                        if (s_i == last) umma_commit(smem_addr(&bars->x_empty));
-                    }
-                    __syncwarp();
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        umma_ss_on(on, tmem + buf * NT,
+                                   lo0 + ((C::kOffX + C::kXTile) >> 4) + (kk >> 2) * (C::kXChunk >> 4) + (kk & 3) * 2,
+                                   y + (C::kYTile >> 4) + (kk >> 2) * (C::kYChunk >> 4) + (kk & 3) * 2, desc_hi, kIdescS,
+                                   kk > 0);
+                    umma_commit_on(on, smem_addr(&bars->dp_full[buf]));
+                    if (s == last) umma_commit_on(on, smem_addr(&bars->x_empty));
                 } else {
-                    if (!(ok = warp_wait(smem_addr(&bars->p_ready[buf]), (n >> 1) & 1u, ctl, kSiteAccP))) break;
-                    if (s_i == 0 && n_it > 0 &&
+                    if (!(ok = warp_wait(smem_addr(&bars->p_ready[buf]), use & 1u, ctl, kSiteAccP))) break;
+                    if (s == 0 && n_it > 0 &&
                         !(ok = warp_wait(smem_addr(&bars->acc_free), (uint32_t)(n_it - 1) & 1u, ctl, kSiteAccFree)))
                         break;
                     tc_fence_after();
-                    if (leader && s_i >= lead) {
-                        const uint32_t acc = tmem + C::kColAcc;
+                    const uint32_t a_col = tmem + buf * NT, acc = tmem + kColAcc;
+                    const uint32_t ymn = lo0_mn + (C::kOffY >> 4) + st * (2 * C::kYTile >> 4);
+                    const uint32_t act = s >= lead ? on : 0u;
 #pragma unroll
-                        for (int kk = 0; kk < NT / 16; ++kk)
-#pragma unroll
-                            for (int ch = 0; ch < C::kChunks; ++ch) {
-                                const uint32_t off = ch * (C::kYChunk >> 4) + kk * 128;  // 16 rows of 128 bytes
-                                const uint32_t add = (s_i > lead || kk > 0) ? 1u : 0u;
-                                if constexpr (kDQ) {
-                                    umma_ts_lo(acc + ch * 64, tS + kk * 8, y_lo + off, desc_hi, kIdescG, add);
-                                } else {
-                                    umma_ts_lo(acc + ch * 64, tS + kk * 8, y_lo + (C::kYTile >> 4) + off, desc_hi, kIdescG, add);
-                                    umma_ts_lo(acc + D + ch * 64, tS + NT / 2 + kk * 8, y_lo + off, desc_hi, kIdescG, add);
-                                }
-                            }
+                    for (int kk = 0; kk < NT / 16; ++kk) {  // 16 rows of 128 bytes, 8 TMEM columns
+                        const uint32_t add = (s > lead || kk > 0) ? 1u : 0u;
+                        if constexpr (kDQ) {
+                            umma_ts_on(act, acc, a_col + kk * 8, ymn + kk * 128, desc_hi, kIdescG, add);
+                        } else {
+                            umma_ts_on(act, acc, a_col + kk * 8, ymn + (C::kYTile >> 4) + kk * 128, desc_hi, kIdescG, add);
+                            umma_ts_on(act, acc + D, a_col + NT / 2 + kk * 8, ymn + kk * 128, desc_hi, kIdescG, add);
+                        }
                     }
-                    if (leader) {
-                        umma_commit(smem_addr(&bars->s_free[buf]));
-                        umma_commit(smem_addr(&bars->y_empty[st]));
-                        if (s_i == last) umma_commit(smem_addr(&bars->acc_full));
-                    }
-                    __syncwarp();
+                    umma_commit_on(on, smem_addr(&bars->buf_free[buf]));
+                    umma_commit_on(on, smem_addr(&bars->y_empty[st]));
+                    if (s == last) umma_commit_on(on, smem_addr(&bars->acc_full));
                 }
+                __syncwarp();
                 if (++st == C::kStages) {
                     st = 0;
                     par ^= 1u;
@@ -587,8 +615,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++n_it;
         }
         // Drain: every MMA this warp issued has finished before TMEM is released.
-        const uint32_t drain_bar = smem_addr(&bars->drain[front ? 0 : 1]);
-        if (leader) umma_commit(drain_bar);
+        const uint32_t drain_bar = smem_addr(&bars->drain[role]);
+        umma_commit_on(on, drain_bar);
         __syncwarp();
         int never = 0;
         const WaitCtl drain{&never, nullptr, ctl.limit_ns};

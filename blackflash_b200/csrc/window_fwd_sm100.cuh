@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     Bars<D>* bars = reinterpret_cast<Bars<D>*>(smem + C::kOffBar);
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // known to be uniform
     const int lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {

@@ -128,19 +128,20 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     p.nk = (Nkv + 127) / 128;
     p.ns = (p.sinks + 127) / 128;
     p.n_pad = (Nq + 127) / 128 * 128;
-    const int nt = d == 64 ? 128 : 64;
+    const int nt = bfk::winb::NT;
     const long long units = (long long)B * Hkv, group = Hq / Hkv;
     // Steps of a tile that only its window's queries see, and of one that holds sinks.
     const long long seen = (long long)p.window + 127 < Nq ? (long long)p.window + 127 : Nq;
     const long long norm = group * ((seen + nt - 1) / nt), sink = group * ((Nq + nt - 1) / nt);
     const long long total = units * ((p.nk - p.ns) * norm + p.ns * sink);
     // Two items a multiprocessor where the work allows it, none shorter than 16 steps (below
-    // that a part's own fp32 output weighs more than what it reads); a sink tile in parts no
-    // shorter than the other items.
+    // that a part's own fp32 output weighs more than what it reads). The blocks take items in
+    // turn, so a sink tile comes in parts of about the other items' length.
     long long target = (total + 2 * kPlanSms - 1) / (2 * kPlanSms);
     if (target < 16) target = 16;
     p.splits_n = norm * 2 > target * 3 ? (int)((norm + target - 1) / target) : 1;
-    const long long target_s = target > norm ? target : norm;
+    const long long floor_s = target < 64 ? target : 64;
+    const long long target_s = p.splits_n > 1 ? target : (norm > floor_s ? norm : floor_s);
     p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
     // D from fp32 sums where a row sees at most a tile of keys: there the rounding of O would
     // dominate the error of dQ and dK.
@@ -194,7 +195,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     const BwdPlan plan = bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks);
     if (workspace_bytes < plan.bytes)
         return bf_set_error(BF_ERR_ARG, "workspace smaller than blackflash_window_bwd_workspace_bytes()");
-    const int nt = d == 64 ? 128 : 64;
+    const int nt = bfk::winb::NT;
     const int q_tiles = plan.n_pad / 128;
     const long long units = (long long)B * Hkv;
     const long long kv_items = units * ((long long)plan.ns * plan.splits_s + (long long)(plan.nk - plan.ns) * plan.splits_n);
@@ -220,13 +221,15 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
     const long long tq[3] = {sq.s[2], sq.s[1], sq.s[0]}, tk[3] = {sk.s[2], sk.s[1], sk.s[0]},
                     tv[3] = {sv.s[2], sv.s[1], sv.s[0]}, td[3] = {sd.s[2], sd.s[1], sd.s[0]};
-    CUtensorMap mq, mk, mv, md, sq_map, sd_map;  // 128-row boxes; streamed queries in nt-row boxes
-    if ((rc = make_map_4d(&mq, Q->data, false, dq, tq, 128, 1)) != BF_OK) return rc;
-    if ((rc = make_map_4d(&md, dO->data, false, dq, td, 128, 1)) != BF_OK) return rc;
-    if ((rc = make_map_4d(&mk, K->data, false, dk, tk, 128, 1)) != BF_OK) return rc;
-    if ((rc = make_map_4d(&mv, V->data, false, dk, tv, 128, 1)) != BF_OK) return rc;
-    if ((rc = make_map_4d(&sq_map, Q->data, false, dq, tq, nt, 1)) != BF_OK) return rc;
-    if ((rc = make_map_4d(&sd_map, dO->data, false, dq, td, nt, 1)) != BF_OK) return rc;
+    // Stationary tiles in 128-row boxes [0], streamed ones in nt-row boxes [1].
+    CUtensorMap mq[2], mk[2], mv[2], md[2];
+    for (int i = 0; i < 2; ++i) {
+        const int box = i ? nt : 128;
+        if ((rc = make_map_4d(&mq[i], Q->data, false, dq, tq, box, 1)) != BF_OK) return rc;
+        if ((rc = make_map_4d(&md[i], dO->data, false, dq, td, box, 1)) != BF_OK) return rc;
+        if ((rc = make_map_4d(&mk[i], K->data, false, dk, tk, box, 1)) != BF_OK) return rc;
+        if ((rc = make_map_4d(&mv[i], V->data, false, dk, tv, box, 1)) != BF_OK) return rc;
+    }
 
     bfk::winb::Params p;
     memset(&p, 0, sizeof(p));
@@ -255,10 +258,12 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.part = part;
     p.timeout_ns = kTimeoutNs;
     p.items = (int)q_items;  // first: it may leave a better D
-    rc = d == 64 ? launch_bwd<64, true>(mq, md, mk, mv, p, st) : launch_bwd<128, true>(mq, md, mk, mv, p, st);
+    rc = d == 64 ? launch_bwd<64, true>(mq[0], md[0], mk[1], mv[1], p, st)
+                 : launch_bwd<128, true>(mq[0], md[0], mk[1], mv[1], p, st);
     if (rc != BF_OK) return rc;
     p.items = (int)kv_items;
-    rc = d == 64 ? launch_bwd<64, false>(mk, mv, sq_map, sd_map, p, st) : launch_bwd<128, false>(mk, mv, sq_map, sd_map, p, st);
+    rc = d == 64 ? launch_bwd<64, false>(mk[0], mv[0], mq[1], md[1], p, st)
+                 : launch_bwd<128, false>(mk[0], mv[0], mq[1], md[1], p, st);
     if (rc != BF_OK) return rc;
     auto join = [&](const float* from, int j0, int tiles, int splits) -> int {
         if (splits <= 1 || tiles <= 0) return BF_OK;
