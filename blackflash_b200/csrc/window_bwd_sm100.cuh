@@ -33,7 +33,11 @@
 // exponentials run; P and dS, as bf16 the A operands of the accumulations, go over dP. With two
 // buffers a group, no step waits for the accumulations of the step before (with S and dP
 // buffers apart, one each a group, it did: 1970 cycles a step against the tensor core's 1020).
-// P stays fp32 until it is multiplied by dP - D, so that dS is rounded once. 64-row streamed
+// P stays fp32 until it is multiplied by dP - D, so that dS is rounded once. In the dK/dV pass
+// lse and D go by column, the same for all rows: read from shared memory by every thread they
+// took a third of its bandwidth. There the tensor core subtracts them instead: each query has 16
+// bytes more, -lse / scale and -D in three bf16 terms each (24 bits), which one more K = 16
+// product adds to S and to dP against stationary rows of ones and zeros. 64-row streamed
 // tiles leave that room, and 32 columns a thread fit the 104 registers that sixteen
 // elementwise warps can have; the price is that S and dP, 64 wide, are bound by reading their
 // stationary operand from shared memory (48 cycles an MMA instead of 32).
@@ -58,12 +62,15 @@ struct Cfg {
     static constexpr int kXChunk = 128 * 128, kXTile = kChunks * kXChunk;
     static constexpr int kYChunk = NT * 128, kYTile = kChunks * kYChunk;
     static constexpr int kStages = D == 128 ? 4 : 6;
-    static constexpr int kVec = kDQ ? 0 : 2 * NT * 4;  // -lse2 and -D of the streamed queries
+    static constexpr int kVec = kDQ ? 0 : NT * 16;  // dK/dV: a tile's rows of Params::aug
     static constexpr int kOffX = 0;
     static constexpr int kOffY = kOffX + 2 * kXTile;              // [kStages][Y0, Y1]
     static constexpr int kOffVec = kOffY + kStages * 2 * kYTile;  // [kStages]
-    static constexpr int kOffSum = kOffVec + kStages * kVec;      // dQ: [2][2 groups][128] {sum P, sum P dP}
-    static constexpr int kOffBar = kOffSum + (kDQ ? 4096 : 0);
+    // dK/dV: 128 rows of 16 bytes with ones at -D's terms, 128 with ones at -lse's, 128 of
+    // zeros. dQ: [2][2 groups][128] {sum P, sum P dP}.
+    static constexpr int kOffOnes = kOffVec + kStages * kVec;
+    static constexpr int kOffSum = kOffOnes;
+    static constexpr int kOffBar = kOffOnes + (kDQ ? 4096 : 3 * 2048);
     static constexpr int kAccs = kDQ ? 1 : 2;
     static_assert(kColAcc + kAccs * D <= kTmemCols, "TMEM columns");
 };
@@ -115,8 +122,9 @@ struct Params {
     int splits_s, splits_n;  // dK/dV: parts of a sink tile's and of another tile's queries
     float scale, scale_log2;
     const float* nlse2;      // [B Hq, n_pad] -lse log2(e); -inf past n_q and for rows that see nothing
-    float* nd;               // [B Hq, n_pad] -D
-    int two_sweeps;          // dQ: find D in a first sweep over the KV tiles, and store it
+    const float* nd;         // [B Hq, n_pad] -D
+    uint4* aug;              // [B Hq, n_pad] eight bf16: -lse / scale in three terms, -D in three, 0, 0
+    int two_sweeps;          // dQ: find D in a first sweep over the KV tiles, and store it in aug
     __nv_bfloat16 *dq, *dk, *dv;
     float* part;             // [slot][dV, dK][128][D] of the tiles with more than one part
     unsigned long long timeout_ns;
@@ -139,6 +147,15 @@ __device__ __forceinline__ void queries_of(const Params& p, int j, int& i0, int&
     const int hi = j < p.ns ? p.n_q : min(p.n_q, last_key + p.window - off);
     i0 = lo / NT;
     ni = hi > lo ? (hi + NT - 1) / NT - i0 : 0;
+}
+
+// x in three bf16 terms: hi + mid + lo is x to 24 bits.
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    hi = pack_bf16x2(x, 0.f) & 0xffffu;
+    x -= __uint_as_float(hi << 16);
+    mid = pack_bf16x2(x, 0.f) & 0xffffu;
+    x -= __uint_as_float(mid << 16);
+    lo = pack_bf16x2(x, 0.f) & 0xffffu;
 }
 
 template <int D, bool kDQ>
@@ -219,6 +236,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_addr(&bars->sums), kEwWarps);
         bars->abort_flag = 0;
         fence_barrier_init();
+    }
+    if constexpr (!kDQ) {
+        if (threadIdx.x < 384) {
+            const uint32_t one = 0x3f80u;  // bf16
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (threadIdx.x < 128)
+                v = make_uint4(0, one << 16, one | (one << 16), 0);
+            else if (threadIdx.x < 256)
+                v = make_uint4(one | (one << 16), one, 0, 0);
+            *reinterpret_cast<uint4*>(smem + C::kOffOnes + threadIdx.x * 16) = v;
+        }
+        fence_proxy_async_smem();
     }
     if (warp == kProdWarp && lane == 0) {
         tma_prefetch_desc(&tmX0);
@@ -308,31 +337,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) pr[c] = __uint_as_float(s[c]);
                 }
-                const float* vec = reinterpret_cast<const float*>(smem + C::kOffVec + (n % C::kStages) * C::kVec) + h * NC;
-                if constexpr (!kDQ) {
-                    // The vectors came with Y; seen here too, their copy is visible to this warp.
-                    if (!warp_wait(smem_addr(&bars->y_full[n % C::kStages]), (n / C::kStages) & 1u, ctl, kSiteEwS)) return false;
-                }
                 if (last < NC || (first > 0 && snk < NC)) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
                         if (c >= last || (c < first && c >= snk)) pr[c] = -INFINITY;
                 }
 #pragma unroll
-                for (int c = 0; c < NC; c += 4) {
-                    uint64_t a = nl2, b = nl2;
-                    if constexpr (!kDQ) {
-                        const float4 v = *reinterpret_cast<const float4*>(vec + c);
-                        a = f2_pack(v.x, v.y);
-                        b = f2_pack(v.z, v.w);
-                    }
-                    float x0, x1, x2, x3;
-                    f2_unpack(f2_fma(f2_pack(pr[c], pr[c + 1]), sl2_2, a), x0, x1);
-                    f2_unpack(f2_fma(f2_pack(pr[c + 2], pr[c + 3]), sl2_2, b), x2, x3);
+                for (int c = 0; c < NC; c += 2) {
+                    float x0, x1;  // dK/dV: S has its -lse already, nl2 is 0
+                    f2_unpack(f2_fma(f2_pack(pr[c], pr[c + 1]), sl2_2, nl2), x0, x1);
                     pr[c] = fast_exp2(x0);
                     pr[c + 1] = fast_exp2(x1);
-                    pr[c + 2] = fast_exp2(x2);
-                    pr[c + 3] = fast_exp2(x3);
                 }
                 // dS = P (dP - D)
                 if (!warp_wait(smem_addr(&bars->dp_full[buf]), par, ctl, kSiteEwDP)) return false;
@@ -349,26 +364,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_st16x32bx2_x16<NC / 2>(tB, pk);
                 }
 #pragma unroll
-                for (int c = 0; c < NC; c += 4) {
-                    uint64_t a = nd2, b = nd2;
-                    if constexpr (!kDQ) {
-                        const float4 v = *reinterpret_cast<const float4*>(vec + NT + c);
-                        a = f2_pack(v.x, v.y);
-                        b = f2_pack(v.z, v.w);
-                    }
-                    float x0, x1, x2, x3;
-                    f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), a), x0, x1);
-                    f2_unpack(f2_add(f2_pack(__uint_as_float(dp[c + 2]), __uint_as_float(dp[c + 3])), b), x2, x3);
-                    x0 *= pr[c];
-                    x1 *= pr[c + 1];
-                    x2 *= pr[c + 2];
-                    x3 *= pr[c + 3];
+                for (int c = 0; c < NC; c += 2) {
+                    uint64_t x = f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1]));
+                    if constexpr (kDQ) x = f2_add(x, nd2);  // dK/dV: dP has its -D already
+                    float x0, x1;
+                    f2_unpack(f2_mul(x, f2_pack(pr[c], pr[c + 1])), x0, x1);
                     if (kDQ && measure) {  // D is 0 so far: x is P dP
-                        sum_p += (pr[c] + pr[c + 1]) + (pr[c + 2] + pr[c + 3]);
-                        sum_pdp += (x0 + x1) + (x2 + x3);
+                        sum_p += pr[c] + pr[c + 1];
+                        sum_pdp += x0 + x1;
                     }
                     pk[c / 2] = pack_bf16x2(x0, x1);
-                    pk[c / 2 + 1] = pack_bf16x2(x2, x3);
                 }
                 if (!measure) {
                     tmem_st16x32bx2_x16<NC / 2>(tB + (kDQ ? 0 : NT / 2), pk);
@@ -396,7 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float tp = x.x + y.x, tpdp = x.y + y.y;
                     const float b = tp != 0.f ? -tpdp / tp : 0.f;  // a row that sees nothing has D = 0
                     nd2 = f2_pack(b, b);
-                    if (grp == 0 && h == 0) p.nd[((size_t)it.b * p.hq + it.head) * p.n_pad + xrow] = b;
+                    if (grp == 0 && h == 0) {
+                        uint32_t d0, d1, d2;
+                        split3(b, d0, d1, d2);
+                        uint32_t* a = reinterpret_cast<uint32_t*>(p.aug + ((size_t)it.b * p.hq + it.head) * p.n_pad + xrow);
+                        reinterpret_cast<uint16_t*>(a)[3] = (uint16_t)d0;
+                        a[2] = d1 | (d2 << 16);
+                    }
                 }
             }
             if constexpr (!kDQ) q_tile = it.ni > 0 ? (it.s0 + s_all) % it.ni : 0;
@@ -508,8 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if constexpr (!kDQ) {
                         const size_t at = ((size_t)it.b * p.hq + head) * p.n_pad + yrow;
-                        bulk_load(vec0 + st * C::kVec, p.nlse2 + at, NT * 4, f);
-                        bulk_load(vec0 + st * C::kVec + NT * 4, p.nd + at, NT * 4, f);
+                        bulk_load(vec0 + st * C::kVec, p.aug + at, C::kVec, f);
                     }
                 }
                 __syncwarp();
@@ -543,6 +553,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t desc_hi = (uint32_t)(desc_base >> 32);
         const uint32_t lo0 = (uint32_t)desc_base;
         const uint32_t lo0_mn = (uint32_t)smem_desc_sw128(smem_addr(smem), C::kYChunk, 1024);
+        // The rows of -lse and -D terms: K-major without swizzle, 8-row groups 128 bytes apart. The
+        // ones have their zeros (K 8..15) a leading-dimension step away; the streamed rows have
+        // none, their step is 0: against those zeros any finite value will do.
+        const uint32_t aug_hi = (uint32_t)((128 >> 4) | (1u << 14));
+        const uint32_t ones_d = (smem_addr(smem + C::kOffOnes) >> 4) | ((4096u >> 4) << 16);
+        const uint32_t ones_s = ((smem_addr(smem + C::kOffOnes) + 2048) >> 4) | ((2048u >> 4) << 16);
+        const uint32_t vec_lo = smem_addr(smem + C::kOffVec) >> 4;
         const int role = warp - kFrontWarp;  // 0 S, 1 dP, 2 accumulations
         uint32_t n = 0, st = 0, par = 0;     // step, its stage and the stage's parity
         int n_it = 0;
@@ -568,6 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int kk = 0; kk < D / 16; ++kk)
                         umma_ss_on(on, tmem + buf * NT, lo0 + (C::kOffX >> 4) + (kk >> 2) * (C::kXChunk >> 4) + (kk & 3) * 2,
                                    y + (kk >> 2) * (C::kYChunk >> 4) + (kk & 3) * 2, desc_hi, kIdescS, kk > 0);
+                    if constexpr (!kDQ) umma_ss_on(on, tmem + buf * NT, ones_s, vec_lo + st * (C::kVec >> 4), aug_hi, kIdescS, 1);
                     umma_commit_on(on, smem_addr(&bars->s_full[buf]));
                     if (s == last) umma_commit_on(on, smem_addr(&bars->x_empty));
                 } else if (role == 1) {
@@ -581,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    lo0 + ((C::kOffX + C::kXTile) >> 4) + (kk >> 2) * (C::kXChunk >> 4) + (kk & 3) * 2,
                                    y + (C::kYTile >> 4) + (kk >> 2) * (C::kYChunk >> 4) + (kk & 3) * 2, desc_hi, kIdescS,
                                    kk > 0);
+                    if constexpr (!kDQ) umma_ss_on(on, tmem + buf * NT, ones_d, vec_lo + st * (C::kVec >> 4), aug_hi, kIdescS, 1);
                     umma_commit_on(on, smem_addr(&bars->dp_full[buf]));
                     if (s == last) umma_commit_on(on, smem_addr(&bars->x_empty));
                 } else {
@@ -632,16 +651,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// -lse log2(e) and -D, D_r = sum_c dO_rc O_rc, over [B Hq, n_pad]. Padded rows and rows that
-// saw nothing (lse = -inf) get -inf, so that exp2(s + that) = 0. Eight lanes a row of 64.
+// -lse log2(e), -D, D_r = sum_c dO_rc O_rc, and both as terms (Params::aug), over [B Hq, n_pad].
+// Padded rows and rows that saw nothing (lse = -inf) get -inf, and as a term -10^37 (times 0
+// it stays 0), so that their weights are 0. D / 8 lanes a row, 16 bytes each.
 template <int D>
 __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restrict__ o, const char* __restrict__ dout,
                                                    long long sb, long long sh, long long sn, const float* __restrict__ lse,
-                                                   float* __restrict__ nlse2, float* __restrict__ nd, int hq, int n,
-                                                   int n_pad, long long rows, int with_d) {
+                                                   float* __restrict__ nlse2, float* __restrict__ nd, uint4* __restrict__ aug,
+                                                   float inv_scale, int hq, int n, int n_pad, long long rows, int with_d) {
     griddep_launch_dependents();
     griddep_wait();
-    constexpr int L = D / 8;  // lanes of a row, 16 bytes each
+    constexpr int L = D / 8;
     const int lane = threadIdx.x % L;
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
     const bool live = r < rows;
@@ -663,8 +683,13 @@ __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restri
     for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
     if (live && lane == 0) {
         const float l = in ? lse[bh * n + i] : -INFINITY;
-        nlse2[r] = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
+        const bool seen = l != -INFINITY;
+        nlse2[r] = seen ? -l * 1.4426950408889634f : -INFINITY;
         nd[r] = -acc;
+        uint32_t l0, l1, l2, d0, d1, d2;
+        split3(seen ? -l * inv_scale : -1e37f, l0, l1, l2);
+        split3(-acc, d0, d1, d2);
+        aug[r] = make_uint4(l0 | (l1 << 16), l2 | (d0 << 16), d1 | (d2 << 16), 0u);
     }
 }
 

@@ -10,8 +10,7 @@
 // range and its log2-sum-exp2, joined later.
 //
 // The roles, TMEM use and softmax are those of the dense kernels beside it (16 softmax
-// warps with two threads per row, a TMA producer, an S issuer and a PV issuer, persistent
-// CTAs). What differs:
+// warps with two threads per row, a TMA producer, issuers, persistent CTAs). What differs:
 //   * an item is two 128-row query tiles of one KV head, each with a list of KV tiles of
 //     its own. With an even group the two are two heads at the same rows, so both lists
 //     are the same and K/V are read once for both; otherwise they are two consecutive row
@@ -28,8 +27,8 @@ namespace win {
 
 constexpr int kSoftWarps = 16;     // 8 per query tile
 constexpr int kProducerWarp = 16;  // TMA producer
-constexpr int kSWarp = 17;         // issues S = Q K^T; owns the TMEM allocation
-constexpr int kPVWarp = 18;        // issues O += P V; warp 19 completes the warpgroup
+constexpr int kSWarp = 17;         // issues S = Q K^T of query tile 0, warp 19 of tile 1; owns the TMEM allocation
+constexpr int kPVWarp = 18;        // issues O += P V
 constexpr int kThreads = 20 * 32;
 constexpr int kTmemCols = 512;
 // Launch budget 96 x 640 = 61440 registers: 104 x 512 + 64 x 128.
@@ -69,8 +68,7 @@ struct Bars {
     uint64_t s_empty[2];
     uint64_t p_full[2];
     uint64_t pv_done[2];
-    uint64_t drain;
-    uint64_t drain_pv;
+    uint64_t drain[3];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -201,11 +199,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < C::kQBufs; ++b) {
             mbar_init(smem_addr(&bars->q_full[b][0]), 1);
             mbar_init(smem_addr(&bars->q_full[b][1]), 1);
-            mbar_init(smem_addr(&bars->q_empty[b]), 1);
+            mbar_init(smem_addr(&bars->q_empty[b]), 2);  // one arrival per S issuer
         }
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(smem_addr(&bars->k_full[s]), 1);
-            mbar_init(smem_addr(&bars->k_empty[s]), 1);
+            mbar_init(smem_addr(&bars->k_empty[s]), 2);
             mbar_init(smem_addr(&bars->v_full[s]), 1);
             mbar_init(smem_addr(&bars->v_empty[s]), 1);
         }
@@ -215,8 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_addr(&bars->p_full[t]), 8);
             mbar_init(smem_addr(&bars->pv_done[t]), 1);
         }
-        mbar_init(smem_addr(&bars->drain), 1);
-        mbar_init(smem_addr(&bars->drain_pv), 1);
+        for (int r = 0; r < 3; ++r) mbar_init(smem_addr(&bars->drain[r]), 1);
         bars->abort_flag = 0;
         fence_barrier_init();
     }
@@ -531,25 +528,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   (uint32_t)((last_q - s) / C::kQBufs) & 1u, drain, 0);
         }
         __syncwarp();
-    } else if (warp == kSWarp || warp == kPVWarp) {
+    } else {
         // ------------------------------------------------------------ MMA issuers
         constexpr uint32_t kFmt = kF16 ? ~((1u << 7) | (1u << 10)) : ~0u;  // A and B format bits: 0 = fp16, 1 = bf16
         constexpr uint32_t kIdescS = idesc_bf16_f32(128, 128, 0) & kFmt;
         constexpr uint32_t kIdescSh = idesc_bf16_f32(128, 64, 0) & kFmt;
         constexpr uint32_t kHalfRowsLo = (64 * 128) >> 4;  // K rows 64.. inside a chunk
         constexpr uint32_t kIdescO = idesc_bf16_f32(128, 64, 1) & kFmt;
-        const bool leader = elect_one();
-        const uint64_t desc_base = smem_desc_sw128(smem_addr(smem), 16, 1024);
-        const uint32_t desc_hi = (uint32_t)(desc_base >> 32);
-        const uint32_t desc_lo0 = (uint32_t)desc_base;
         constexpr uint32_t kChunkLo = C::kChunkBytes >> 4;
         constexpr uint32_t kTileLo = C::kTile >> 4;
-        const uint32_t q_lo0 = desc_lo0 + (C::kOffQ >> 4), k_lo0 = desc_lo0 + (C::kOffK >> 4),
-                       v_lo0 = desc_lo0 + (C::kOffV >> 4);
-        const bool is_s = warp == kSWarp;
-        uint32_t g[2] = {0, 0};  // steps of tile t so far
-        int st = 0, n_it = 0;
-        uint32_t par = 0;
+        const uint32_t on = elect_one() ? 1u : 0u;
+        const uint64_t desc_base = smem_desc_sw128(smem_addr(smem), 16, 1024);
+        const uint32_t desc_hi = (uint32_t)(desc_base >> 32);
+        const uint32_t lo0 = (uint32_t)desc_base;
+        const uint32_t v_lo0 = lo0 + (C::kOffV >> 4);
+        const bool is_pv = warp == kPVWarp;
+        const int ts = warp == kSWarp ? 0 : 1;  // S issuers: their tile
+        uint32_t g[2] = {0, 0};                 // steps of tile t so far
+        uint32_t st = 0, par = 0;
+        int n_it = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
             Item it;
@@ -558,92 +555,68 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int qb = n_it % C::kQBufs;
             const uint32_t q_par = (uint32_t)(n_it / C::kQBufs) & 1u;
             ++n_it;
-            const uint32_t g0[2] = {g[0], g[1]};
+            bool first[2] = {true, true};
             for (int s_i = 0; s_i < it.steps; ++s_i) {
                 const int j = step_tile(it, s_i);
-                if (is_s) {
+                if (!is_pv) {
                     if (!(ok = warp_wait(smem_addr(&bars->k_full[st]), par, ctl, kSiteMmaK))) break;
-                    tc_fence_after();
-                    const uint32_t k_lo = k_lo0 + (uint32_t)st * kTileLo;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (s_i == 0) {  // both tiles, idle ones too: their loads must land before the buffer is reused
-                            if (!(ok = warp_wait(smem_addr(&bars->q_full[qb][t]), q_par, ctl, kSiteMmaQ + t))) break;
-                            tc_fence_after();
-                        }
-                        if (!sees(p, it, t, j)) continue;
-                        const uint32_t q_lo = q_lo0 + (uint32_t)(qb * 2 + t) * kTileLo;
-                        if (g[t] > 0) {
-                            if (!(ok = warp_wait(smem_addr(&bars->s_empty[t]), (g[t] - 1) & 1u, ctl, kSiteMmaK + 3 + t)))
-                                break;
-                            tc_fence_after();
-                        }
+                    // An idle tile's query load, too, must land before its buffer is reused.
+                    if (s_i == 0 && !(ok = warp_wait(smem_addr(&bars->q_full[qb][ts]), q_par, ctl, kSiteMmaQ + ts))) break;
+                    if (sees(p, it, ts, j)) {
+                        const uint32_t k_lo = lo0 + (C::kOffK >> 4) + st * kTileLo;
+                        const uint32_t q_lo = lo0 + (C::kOffQ >> 4) + (uint32_t)(qb * 2 + ts) * kTileLo;
+                        const uint32_t d = tmem + ts * 128;
+                        if (g[0] > 0 && !(ok = warp_wait(smem_addr(&bars->s_empty[ts]), (g[0] - 1) & 1u, ctl, kSiteMmaK + 3 + ts)))
+                            break;
+                        tc_fence_after();
                         if constexpr (C::kSepP) {
-                            if (leader) {
 #pragma unroll
-                                for (int kk = 0; kk < D / 16; ++kk)
-                                    umma_ss_lo(tmem + t * 128, q_lo + kk * 2, k_lo + kk * 2, desc_hi, kIdescS, kk > 0);
-                                umma_commit(smem_addr(&bars->s_full[t]));
-                            }
+                            for (int kk = 0; kk < D / 16; ++kk)
+                                umma_ss_on(on, d, q_lo + kk * 2, k_lo + kk * 2, desc_hi, kIdescS, kk > 0);
                         } else {
                             // Keys 64..127 as soon as S_t has been loaded; keys 0..63, where P_t lives,
                             // after PV_t of the previous step has read P_t.
-                            if (leader) {
 #pragma unroll
-                                for (int kk = 0; kk < D / 16; ++kk) {
-                                    const uint32_t off = (uint32_t)(kk >> 2) * kChunkLo + (uint32_t)(kk & 3) * 2;
-                                    umma_ss_lo(tmem + t * 128 + 64, q_lo + off, k_lo + off + kHalfRowsLo, desc_hi, kIdescSh,
-                                               kk > 0);
-                                }
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t off = (uint32_t)(kk >> 2) * kChunkLo + (uint32_t)(kk & 3) * 2;
+                                umma_ss_on(on, d + 64, q_lo + off, k_lo + off + kHalfRowsLo, desc_hi, kIdescSh, kk > 0);
                             }
-                            __syncwarp();
-                            if (g[t] > 0) {
-                                if (!(ok = warp_wait(smem_addr(&bars->pv_done[t]), (g[t] - 1) & 1u, ctl,
-                                                     kSiteMmaK + 1 + t)))
-                                    break;
-                                tc_fence_after();
-                            }
-                            if (leader) {
+                            if (g[0] > 0 &&
+                                !(ok = warp_wait(smem_addr(&bars->pv_done[ts]), (g[0] - 1) & 1u, ctl, kSiteMmaK + 1 + ts)))
+                                break;
+                            tc_fence_after();
 #pragma unroll
-                                for (int kk = 0; kk < D / 16; ++kk) {
-                                    const uint32_t off = (uint32_t)(kk >> 2) * kChunkLo + (uint32_t)(kk & 3) * 2;
-                                    umma_ss_lo(tmem + t * 128, q_lo + off, k_lo + off, desc_hi, kIdescSh, kk > 0);
-                                }
-                                umma_commit(smem_addr(&bars->s_full[t]));
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t off = (uint32_t)(kk >> 2) * kChunkLo + (uint32_t)(kk & 3) * 2;
+                                umma_ss_on(on, d, q_lo + off, k_lo + off, desc_hi, kIdescSh, kk > 0);
                             }
                         }
-                        ++g[t];
-                        __syncwarp();
+                        umma_commit_on(on, smem_addr(&bars->s_full[ts]));
+                        ++g[0];
                     }
-                    if (!ok) break;
-                    if (leader) {
-                        umma_commit(smem_addr(&bars->k_empty[st]));
-                        if (s_i == it.steps - 1) umma_commit(smem_addr(&bars->q_empty[qb]));
-                    }
+                    umma_commit_on(on, smem_addr(&bars->k_empty[st]));
+                    if (s_i == it.steps - 1) umma_commit_on(on, smem_addr(&bars->q_empty[qb]));
                     __syncwarp();
                 } else {
                     if (!(ok = warp_wait(smem_addr(&bars->v_full[st]), par, ctl, kSiteMmaV))) break;
-                    const uint32_t v_lo = v_lo0 + (uint32_t)st * kTileLo;
+                    const uint32_t v_lo = v_lo0 + st * kTileLo;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (!sees(p, it, t, j)) continue;
                         if (!(ok = warp_wait(smem_addr(&bars->p_full[t]), g[t] & 1u, ctl, kSiteMmaV + 1 + t))) break;
                         tc_fence_after();
-                        if (leader) {
 #pragma unroll
-                            for (int kk = 0; kk < 8; ++kk)
+                        for (int kk = 0; kk < 8; ++kk)  // 16 keys: 8 TMEM columns of P, 16 x 128 bytes of V
 #pragma unroll
-                                for (int ch = 0; ch < C::kChunks; ++ch)
-                                    umma_ts_lo(tmem + C::kColO + t * D + ch * 64, tmem + C::kColP + t * C::kStepP + kk * 8,
-                                               v_lo + ch * kChunkLo + kk * 128, desc_hi, kIdescO,
-                                               (g[t] > g0[t] || kk > 0) ? 1u : 0u);
-                            umma_commit(smem_addr(&bars->pv_done[t]));
-                        }
+                            for (int ch = 0; ch < C::kChunks; ++ch)
+                                umma_ts_on(on, tmem + C::kColO + t * D + ch * 64, tmem + C::kColP + t * C::kStepP + kk * 8,
+                                           v_lo + ch * kChunkLo + kk * 128, desc_hi, kIdescO, !first[t] || kk > 0);
+                        umma_commit_on(on, smem_addr(&bars->pv_done[t]));
+                        first[t] = false;
                         ++g[t];
-                        __syncwarp();
                     }
                     if (!ok) break;
-                    if (leader) umma_commit(smem_addr(&bars->v_empty[st]));
+                    umma_commit_on(on, smem_addr(&bars->v_empty[st]));
                     __syncwarp();
                 }
                 if (++st == C::kStages) {
@@ -653,8 +626,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // Drain: every MMA this warp issued has finished before TMEM is released.
-        const uint32_t drain_bar = smem_addr(is_s ? &bars->drain : &bars->drain_pv);
-        if (leader) umma_commit(drain_bar);
+        const uint32_t drain_bar = smem_addr(&bars->drain[warp - kSWarp]);
+        umma_commit_on(on, drain_bar);
         __syncwarp();
         int never = 0;
         const WaitCtl drain{&never, nullptr, ctl.limit_ns};

@@ -57,7 +57,7 @@ int check_window(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     if (d != 64 && d != 128) return bf_set_error(BF_ERR_ARG, "BlackFlash supports d=64 and d=128");
     if (Nq > (1 << 30) || Nkv > (1 << 30)) return bf_set_error(BF_ERR_ARG, "more than 2^30 rows");
     if (window < 1 || sinks < 0) return bf_set_error(BF_ERR_ARG, "need window >= 1 and sinks >= 0");
-    if (!(scale > 0.f) || !isfinite(scale)) return bf_set_error(BF_ERR_ARG, "scale must be positive and finite");
+    if (!(scale >= 1e-30f) || !isfinite(scale)) return bf_set_error(BF_ERR_ARG, "scale must be positive (at least 1e-30) and finite");
     return BF_OK;
 }
 
@@ -114,7 +114,7 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
 
 namespace {
 
-// How the dK/dV pass is split, and its workspace: -lse2 and -D, then the parts.
+// How the dK/dV pass is split, and its workspace: -lse2 and -D, both as terms, then the parts.
 struct BwdPlan {
     int nk, ns, window, sinks, n_pad, splits_s, splits_n;
     long long vec, slots, bytes;
@@ -149,7 +149,7 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     p.vec = (long long)B * Hq * p.n_pad;
     p.slots = units * ((p.splits_s > 1 ? (long long)p.ns * p.splits_s : 0) +
                        (p.splits_n > 1 ? (long long)(p.nk - p.ns) * p.splits_n : 0));
-    p.bytes = 4 * (2 * p.vec + p.slots * 2 * 128 * d);
+    p.bytes = 4 * (6 * p.vec + p.slots * 2 * 128 * d);
     return p;
 }
 
@@ -208,14 +208,15 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     float* nlse2 = reinterpret_cast<float*>(workspace);
     float* nd = nlse2 + plan.vec;
-    float* part = nd + plan.vec;
+    uint4* aug = reinterpret_cast<uint4*>(nd + plan.vec);  // vec is a multiple of 128: 16-byte aligned
+    float* part = reinterpret_cast<float*>(aug + plan.vec);
     {
         const int per = 256 / (d / 8);
         const unsigned grid = (unsigned)((plan.vec + per - 1) / per);
         auto kernel = d == 64 ? bfk::winb::prep_kernel<64> : bfk::winb::prep_kernel<128>;
         if ((rc = launch_error(launch_pdl(kernel, dim3(grid), 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
                                           reinterpret_cast<const char*>(dO->data), sd.s[0] * 2, sd.s[1] * 2, sd.s[2] * 2, lse,
-                                          nlse2, nd, Hq, Nq, plan.n_pad, plan.vec, plan.two_sweeps ? 0 : 1))) != BF_OK)
+                                          nlse2, nd, aug, 1.f / scale, Hq, Nq, plan.n_pad, plan.vec, plan.two_sweeps ? 0 : 1))) != BF_OK)
             return rc;
     }
     const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
@@ -252,6 +253,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.scale_log2 = scale * kLog2e;
     p.nlse2 = nlse2;
     p.nd = nd;
+    p.aug = aug;
     p.dq = reinterpret_cast<__nv_bfloat16*>(dQ);
     p.dk = reinterpret_cast<__nv_bfloat16*>(dK);
     p.dv = reinterpret_cast<__nv_bfloat16*>(dV);

@@ -26,9 +26,9 @@ def lib():
 def test_window_backward_plans(lib, change):
     ok = dict(B=1, Hq=4, Hkv=2, Nq=300, Nkv=300, d=64, window=50, sinks=0)
     ws = lib.blackflash_window_bwd_workspace_bytes
-    assert ws(*ok.values()) == 4 * 2 * 4 * 384            # two vectors of 4 heads, 300 rows padded to 384
+    assert ws(*ok.values()) == 4 * 6 * 4 * 384            # six words a row of 4 heads, 300 rows padded to 384
     # Sinks that 100 query tiles see come in parts: 128-row fp32 pieces of dV and dK.
-    many = ws(*{**ok, "Nq": 12800, "Nkv": 12800, "sinks": 4}.values()) - 4 * 2 * 4 * 12800
+    many = ws(*{**ok, "Nq": 12800, "Nkv": 12800, "sinks": 4}.values()) - 4 * 6 * 4 * 12800
     assert many > 0 and many % (2 * 128 * 64 * 4) == 0
     assert ws(*{**ok, **change}.values()) == -1 and lib.blackflash_last_error()
 
