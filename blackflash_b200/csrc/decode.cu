@@ -52,6 +52,7 @@ struct Params {
     int hkv, q_rows, tokens, cap, row_tiles;
     int window, sinks;  // clamped to cap
     int chunk;          // keys of a split
+    int beside;         // the grid before is the prefix part: do not wait for it at the start
     float scale_log2;
 };
 
@@ -107,8 +108,11 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     const int rt = blockIdx.x % p.row_tiles;
     const int bh = blockIdx.x / p.row_tiles;
     const int kvh = bh % p.hkv, b = bh / p.hkv;
+    // Behind the prefix part, this grid was launched only after every grid before that one had
+    // completed, and needs nothing of it. But its own completion, for which the join waits,
+    // has to mean the prefix part's too: the last block waits for it at its end.
     griddep_launch_dependents();
-    griddep_wait();
+    if (!p.beside) griddep_wait();
 
     const int len = min(max(p.lengths[b], 0), p.cap);
     const int pos0 = len - p.tokens;  // position of new token 0; may be negative
@@ -328,6 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
             if (col == 0 && p.lse) p.lse[row] = lse2 * 0.69314718055994531f;
         }
     }
+    if (p.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) griddep_wait();
 }
 
 struct CombineParams {
@@ -553,6 +558,7 @@ int decode_step(const StepArgs& a) {
         p.window = a.window < a.C ? a.window : a.C;
         p.sinks = a.sinks < a.C ? a.sinks : a.C;
         p.chunk = plan.chunk;
+        p.beside = a.P > 0;
         p.scale_log2 = a.scale * kLog2e;
         const long long units = (long long)a.B * a.Hkv * plan.row_tiles;
         if (a.d == 64)

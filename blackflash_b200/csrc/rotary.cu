@@ -59,6 +59,7 @@ struct __align__(sizeof(T) * V) Vec {
 };
 
 constexpr int kBlock = 256;
+constexpr int kMaxTile = 8;      // tokens of a block
 constexpr int kMaxPairs = 512;  // (token, pair) entries of a block's table
 
 // A work item is V consecutive columns of one row: of the first half with their partners of
@@ -66,15 +67,21 @@ constexpr int kMaxPairs = 512;  // (token, pair) entries of a block's table
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kBlock) rotary_kernel(const Params p) {
     __shared__ float2 cs[kMaxPairs];
+    __shared__ int tok_b[kMaxTile], tok_n[kMaxTile];
     const int half = p.rot / 2;
     const long long t0 = (long long)blockIdx.x * p.tile;
     const int nt = (int)min((long long)p.tile, p.tokens - t0);
     griddep_launch_dependents();
     griddep_wait();
+    if (threadIdx.x < nt) {
+        const long long tok = t0 + threadIdx.x, b = tok / p.n;
+        tok_b[threadIdx.x] = (int)b;
+        tok_n[threadIdx.x] = (int)(tok - b * p.n);
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < nt * half; i += kBlock) {
         const int t = i / half, pr = i - t * half;
-        const long long tok = t0 + t;
-        const long long b = tok / p.n, at = b * p.pos_stride + (tok - b * p.n);
+        const long long at = tok_b[t] * p.pos_stride + tok_n[t];
         const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
                                       : (long long)reinterpret_cast<const int*>(p.positions)[at];
         const double turns = (double)pos * (p.freqs[pr] * 0.15915494309189533577);
@@ -88,54 +95,73 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(const Params p) {
     }
     __syncthreads();
 
-    // Items of a row: the rotated ones, then the copied ones.
+    // Items of a row: the rotated ones, then the copied ones. A thread keeps its item and steps
+    // through the rows (token, head) of the block, kAhead of them at a time with all loads
+    // before the first product, so that enough bytes are in flight.
     const int rot_items = kInterleaved ? p.rot / V : half / V;
     const int row_items = rot_items + (p.d - p.rot) / V;
     const int all_heads = p.heads[0] + p.heads[1];
     const int h0 = (int)((long long)all_heads * blockIdx.y / p.head_split);
-    const int h1 = (int)((long long)all_heads * (blockIdx.y + 1) / p.head_split);
-    const int per_token = (h1 - h0) * row_items;
+    const int nh = (int)((long long)all_heads * (blockIdx.y + 1) / p.head_split) - h0;
+    const int across = min(row_items, kBlock), pass = kBlock / across;  // rows of a pass
+    const int first = threadIdx.x / across;
+    if (first >= pass) return;
     using VT = Vec<T, V>;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < nt * per_token; i += kBlock) {
-        const int t = i / per_token;
-        const int rest = i - t * per_token;
-        const int hh = h0 + rest / row_items, item = rest % row_items;
-        const int which = hh >= p.heads[0];
-        const int h = which ? hh - p.heads[0] : hh;
-        const long long tok = t0 + t;
-        const long long b = tok / p.n, n = tok - b * p.n;
-        const T* x = reinterpret_cast<const T*>(p.x[which] + b * p.xs[which][0] + h * p.xs[which][1] + n * p.xs[which][2]);
-        T* y = reinterpret_cast<T*>(p.y[which]) + ((b * p.heads[which] + h) * p.n + n) * p.d;
-        const float2* tab = cs + t * half;
-        if (item >= rot_items) {
-            const int c = p.rot + (item - rot_items) * V;
-            *reinterpret_cast<VT*>(y + c) = *reinterpret_cast<const VT*>(x + c);
-        } else if constexpr (kInterleaved) {
-            const int c = item * V;
-            const VT a = *reinterpret_cast<const VT*>(x + c);
-            VT r;
+    constexpr int kAhead = 4;
+    for (int item = threadIdx.x - first * across; item < row_items; item += kBlock) {
+        const bool turned = item < rot_items;
+        const int col = turned ? item * V : p.rot + (item - rot_items) * V;
+        const int pair = kInterleaved ? col >> 1 : col;
+        int t = first / nh, h = first - t * nh;
+        while (t < nt) {
+            VT a[kAhead], c[kAhead];
+            T* dst[kAhead];
+            const float2* tab[kAhead];
+            int live = 0;
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 w = tab[(c + e) >> 1];
-                const float u = to_f<T>(a.e[e]), v = to_f<T>(a.e[e + 1]);
-                r.e[e] = from_f<T>(u * w.x - v * w.y);
-                r.e[e + 1] = from_f<T>(u * w.y + v * w.x);
+            for (int k = 0; k < kAhead; ++k) {
+                if (t < nt) {
+                    const int hh = h0 + h, which = hh >= p.heads[0], hw = which ? hh - p.heads[0] : hh;
+                    const long long b = tok_b[t], n = tok_n[t];
+                    const T* x = reinterpret_cast<const T*>(p.x[which] + b * p.xs[which][0] + hw * p.xs[which][1] +
+                                                            n * p.xs[which][2]) + col;
+                    dst[k] = reinterpret_cast<T*>(p.y[which]) + ((b * p.heads[which] + hw) * p.n + n) * p.d + col;
+                    tab[k] = cs + t * half + pair;
+                    a[k] = *reinterpret_cast<const VT*>(x);
+                    if (!kInterleaved && turned) c[k] = *reinterpret_cast<const VT*>(x + half);
+                    live = k + 1;
+                    h += pass;
+                    while (h >= nh) {
+                        h -= nh;
+                        ++t;
+                    }
+                }
             }
-            *reinterpret_cast<VT*>(y + c) = r;
-        } else {
-            const int c = item * V;
-            const VT a = *reinterpret_cast<const VT*>(x + c), bq = *reinterpret_cast<const VT*>(x + half + c);
-            VT r, q;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 w = tab[c + e];
-                const float u = to_f<T>(a.e[e]), v = to_f<T>(bq.e[e]);
-                r.e[e] = from_f<T>(u * w.x - v * w.y);
-                q.e[e] = from_f<T>(u * w.y + v * w.x);
+            for (int k = 0; k < kAhead; ++k) {
+                if (k >= live) break;
+                if (turned) {
+                    if constexpr (kInterleaved) {
+#pragma unroll
+                        for (int e = 0; e < V; e += 2) {
+                            const float2 w = tab[k][e >> 1];
+                            const float u = to_f<T>(a[k].e[e]), v = to_f<T>(a[k].e[e + 1]);
+                            a[k].e[e] = from_f<T>(u * w.x - v * w.y);
+                            a[k].e[e + 1] = from_f<T>(u * w.y + v * w.x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const float2 w = tab[k][e];
+                            const float u = to_f<T>(a[k].e[e]), v = to_f<T>(c[k].e[e]);
+                            a[k].e[e] = from_f<T>(u * w.x - v * w.y);
+                            c[k].e[e] = from_f<T>(u * w.y + v * w.x);
+                        }
+                        *reinterpret_cast<VT*>(dst[k] + half) = c[k];
+                    }
+                }
+                *reinterpret_cast<VT*>(dst[k]) = a[k];
             }
-            *reinterpret_cast<VT*>(y + c) = r;
-            *reinterpret_cast<VT*>(y + half + c) = q;
         }
     }
 }
@@ -216,7 +242,7 @@ extern "C" int blackflash_rotary(const bf_view* Q, const bf_view* K, void* Q_out
     // would leave multiprocessors without a block; then the heads are split too.
     int tile = bfk::rot::kBlock / (rotary_dim / 2);
     if (tile < 1) tile = 1;
-    if (tile > 8) tile = 8;
+    if (tile > bfk::rot::kMaxTile) tile = bfk::rot::kMaxTile;
     const long long even = (p.tokens + 2 * kPlanSms - 1) / (2 * kPlanSms);
     if (even < tile) tile = (int)even;
     p.tile = tile;

@@ -654,42 +654,55 @@ __global__ void __launch_bounds__(kThreads, 1)
 // -lse log2(e), -D, D_r = sum_c dO_rc O_rc, and both as terms (Params::aug), over [B Hq, n_pad].
 // Padded rows and rows that saw nothing (lse = -inf) get -inf, and as a term -10^37 (times 0
 // it stays 0), so that their weights are 0. D / 8 lanes a row, 16 bytes each.
+constexpr int kPrepRows = 4;  // rows of a thread
 template <int D>
 __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restrict__ o, const char* __restrict__ dout,
                                                    long long sb, long long sh, long long sn, const float* __restrict__ lse,
                                                    float* __restrict__ nlse2, float* __restrict__ nd, uint4* __restrict__ aug,
-                                                   float inv_scale, int hq, int n, int n_pad, long long rows, int with_d) {
+                                                   float inv_scale, int hq, int n, int n_pad, int with_d) {
     griddep_launch_dependents();
     griddep_wait();
     constexpr int L = D / 8;
+    constexpr int R = 256 / L;  // rows of a block's pass
     const int lane = threadIdx.x % L;
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
-    const bool live = r < rows;
-    const long long bh = live ? r / n_pad : 0;
-    const int i = (int)(r - bh * n_pad);
-    const bool in = live && i < n;
-    float acc = 0.f;
-    if (in && with_d) {
-        const long long b = bh / hq, h = bh - b * hq;
-        const uint4 x = *reinterpret_cast<const uint4*>(o + (bh * n + i) * D + lane * 8);
-        const uint4 y = *reinterpret_cast<const uint4*>(dout + b * sb + h * sh + i * sn + lane * 16);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    const int bh = blockIdx.x, b = bh / hq, h = bh - b * hq;
+    const __nv_bfloat16* o_bh = o + (size_t)bh * n * D + lane * 8;
+    const char* d_bh = dout + b * sb + h * sh + lane * 16;
+    for (int i0 = (int)(blockIdx.y * R * kPrepRows + threadIdx.x / L); i0 < n_pad; i0 += (int)gridDim.y * R * kPrepRows) {
+        // All of a thread's loads before the first sum.
+        uint4 x[kPrepRows], y[kPrepRows];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            acc += __uint_as_float(xs[c] << 16) * __uint_as_float(ys[c] << 16) +
-                   __uint_as_float(xs[c] & 0xffff0000u) * __uint_as_float(ys[c] & 0xffff0000u);
-    }
+        for (int k = 0; k < kPrepRows; ++k) {
+            const int i = i0 + k * R;
+            x[k] = y[k] = make_uint4(0, 0, 0, 0);
+            if (i < n && with_d) {
+                x[k] = *reinterpret_cast<const uint4*>(o_bh + (size_t)i * D);
+                y[k] = *reinterpret_cast<const uint4*>(d_bh + (long long)i * sn);
+            }
+        }
 #pragma unroll
-    for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-    if (live && lane == 0) {
-        const float l = in ? lse[bh * n + i] : -INFINITY;
-        const bool seen = l != -INFINITY;
-        nlse2[r] = seen ? -l * 1.4426950408889634f : -INFINITY;
-        nd[r] = -acc;
-        uint32_t l0, l1, l2, d0, d1, d2;
-        split3(seen ? -l * inv_scale : -1e37f, l0, l1, l2);
-        split3(-acc, d0, d1, d2);
-        aug[r] = make_uint4(l0 | (l1 << 16), l2 | (d0 << 16), d1 | (d2 << 16), 0u);
+        for (int k = 0; k < kPrepRows; ++k) {
+            const int i = i0 + k * R;  // n_pad is a multiple of 128, and so of a pass: all rows or none
+            float acc = 0.f;
+            const uint32_t xs[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                acc += __uint_as_float(xs[c] << 16) * __uint_as_float(ys[c] << 16) +
+                       __uint_as_float(xs[c] & 0xffff0000u) * __uint_as_float(ys[c] & 0xffff0000u);
+#pragma unroll
+            for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
+            if (lane == 0) {
+                const float l = i < n ? lse[(size_t)bh * n + i] : -INFINITY;
+                const bool seen = l != -INFINITY;
+                const size_t r = (size_t)bh * n_pad + i;
+                nlse2[r] = seen ? -l * 1.4426950408889634f : -INFINITY;
+                nd[r] = -acc;
+                uint32_t l0, l1, l2, d0, d1, d2;
+                split3(seen ? -l * inv_scale : -1e37f, l0, l1, l2);
+                split3(-acc, d0, d1, d2);
+                aug[r] = make_uint4(l0 | (l1 << 16), l2 | (d0 << 16), d1 | (d2 << 16), 0u);
+            }
+        }
     }
 }
 

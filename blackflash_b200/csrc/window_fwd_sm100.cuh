@@ -231,9 +231,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
     const WaitCtl ctl{&bars->abort_flag, &g_wait_status, p.timeout_ns};
-    // Nothing above touches global data: it overlaps the previous grid's tail.
-    griddep_launch_dependents();
+    // Nothing above touches global data: it overlaps the previous grid's tail. In partial mode
+    // the next grid is the cache's part of the step, which reads nothing of this one: it may
+    // start, and use the multiprocessors that this grid leaves free, as soon as the grids
+    // before this one are complete.
+    if (!kPartial) griddep_launch_dependents();
     griddep_wait();
+    if (kPartial) griddep_launch_dependents();
 
     if (warp < kSoftWarps)
         regs_inc<kSoftRegs>();

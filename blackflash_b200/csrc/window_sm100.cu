@@ -211,12 +211,13 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     uint4* aug = reinterpret_cast<uint4*>(nd + plan.vec);  // vec is a multiple of 128: 16-byte aligned
     float* part = reinterpret_cast<float*>(aug + plan.vec);
     {
-        const int per = 256 / (d / 8);
-        const unsigned grid = (unsigned)((plan.vec + per - 1) / per);
+        const int per = 256 / (d / 8) * bfk::winb::kPrepRows;  // rows of a block: divides 128
+        const int chunks = plan.n_pad / per;
+        const dim3 grid((unsigned)(B * Hq), (unsigned)(chunks < 65535 ? chunks : 65535));
         auto kernel = d == 64 ? bfk::winb::prep_kernel<64> : bfk::winb::prep_kernel<128>;
-        if ((rc = launch_error(launch_pdl(kernel, dim3(grid), 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
+        if ((rc = launch_error(launch_pdl(kernel, grid, 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
                                           reinterpret_cast<const char*>(dO->data), sd.s[0] * 2, sd.s[1] * 2, sd.s[2] * 2, lse,
-                                          nlse2, nd, aug, 1.f / scale, Hq, Nq, plan.n_pad, plan.vec, plan.two_sweeps ? 0 : 1))) != BF_OK)
+                                          nlse2, nd, aug, 1.f / scale, Hq, Nq, plan.n_pad, plan.two_sweeps ? 0 : 1))) != BF_OK)
             return rc;
     }
     const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
