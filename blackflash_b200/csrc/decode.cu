@@ -202,9 +202,12 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
                 mma16816<kF16>(sc[2 * i + 1], qf[kk], r[2], r[3]);
             }
         }
-        // Mask and scale. With one token every key of the range is visible.
+        // Mask and scale. A group of window keys up to the first token's position and inside the
+        // last one's window, or of sinks, is visible to every row.
         const int vg = v0 + (warp + s * kWarps) * C::kKeys;
-        const bool whole = vg + C::kKeys <= v1 && p.tokens == 1;
+        const int k0 = lo + (vg - s0), k1 = k0 + C::kKeys - 1;
+        const bool whole = vg + C::kKeys <= v1 &&
+                           (vg >= s0 ? k1 <= pos0 && len - 1 - k0 < p.window : vg + C::kKeys <= s0);
         float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -346,46 +349,47 @@ struct CombineParams {
 
 // One block per row, one warp per share of its parts: O = sum_i w_i O_i / sum_i w_i with
 // w_i = 2^(lse_i - max). Parts without a visible key (-inf) are not read.
+constexpr int kJoinWarps = 8;
 template <int D, bool kF16>
-__global__ void __launch_bounds__(128) combine_kernel(const CombineParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const CombineParams p) {
     griddep_wait();
     const long long row = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int E = D / 32;
-    __shared__ float sm_y[4][D], sm_l[4], sm_m[4];
+    __shared__ float sm_y[kJoinWarps][D], sm_l[kJoinWarps], sm_m[kJoinWarps];
     const int total = p.n[0] + p.n[1];
     auto lse_at = [&](int i) {
         return i < p.n[0] ? p.lse[0][(size_t)i * p.rows + row] : p.lse[1][(size_t)(i - p.n[0]) * p.rows + row];
     };
     float m = -INFINITY;
-    for (int i = threadIdx.x; i < total; i += 128) m = fmaxf(m, lse_at(i));
+    for (int i = threadIdx.x; i < total; i += kJoinWarps * 32) m = fmaxf(m, lse_at(i));
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
     if (lane == 0) sm_m[warp] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm_m[w]);
     float y[E], l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < total; i += 4) {
+#pragma unroll 8
+    for (int i = warp; i < total; i += kJoinWarps) {
         const float x = lse_at(i);
         if (x == -INFINITY) continue;
         const float w = fast_exp2(x - m);
         const float* src = (i < p.n[0] ? p.o[0] + ((size_t)i * p.rows + row) * D
                                        : p.o[1] + ((size_t)(i - p.n[0]) * p.rows + row) * D) + lane * E;
         l += w;
+        float a[E];
         if constexpr (E == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(src);
-            y[0] += w * a.x;
-            y[1] += w * a.y;
-            y[2] += w * a.z;
-            y[3] += w * a.w;
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            a[0] = v.x, a[1] = v.y, a[2] = v.z, a[3] = v.w;
         } else {
-            const float2 a = *reinterpret_cast<const float2*>(src);
-            y[0] += w * a.x;
-            y[1] += w * a.y;
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            a[0] = v.x, a[1] = v.y;
         }
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] += w * a[e];
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sm_y[warp][lane * E + e] = y[e];
@@ -393,13 +397,17 @@ __global__ void __launch_bounds__(128) combine_kernel(const CombineParams p) {
     __syncthreads();
     if (threadIdx.x < D / 2) {
         const int c = threadIdx.x * 2;
-        const float sum = sm_l[0] + sm_l[1] + sm_l[2] + sm_l[3];
-        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // NaN stays NaN
-        const float a = (sm_y[0][c] + sm_y[1][c] + sm_y[2][c] + sm_y[3][c]) * inv;
-        const float b = (sm_y[0][c + 1] + sm_y[1][c + 1] + sm_y[2][c + 1] + sm_y[3][c + 1]) * inv;
-        reinterpret_cast<uint32_t*>(p.out)[row * (D / 2) + threadIdx.x] = pack2<kF16>(a, b);
-        if (threadIdx.x == 0 && p.lse_out)
-            p.lse_out[row] = sum > 0.f || sum != sum ? (m + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
+        float sum = 0.f, a = 0.f, b = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            sum += sm_l[w];
+            a += sm_y[w][c];
+            b += sm_y[w][c + 1];
+        }
+        const bool any = sum > 0.f || sum != sum;  // NaN stays NaN
+        const float inv = any ? 1.f / sum : 0.f;
+        reinterpret_cast<uint32_t*>(p.out)[row * (D / 2) + threadIdx.x] = pack2<kF16>(a * inv, b * inv);
+        if (threadIdx.x == 0 && p.lse_out) p.lse_out[row] = any ? (m + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
     }
 }
 
@@ -438,20 +446,38 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
     // The longest run of keys a row tile can see.
     long long vis = (long long)window + T - 1 + sinks;
     if (vis > C) vis = C;
-    // About four blocks of work per slot (two a multiprocessor), so that ragged lengths even
-    // out; at least 128 keys, below which a block is all start-up and join.
-    long long chunk = (vis * units + kPlanSms * 8 - 1) / (kPlanSms * 8);
-    chunk = (chunk + 127) / 128 * 128;
-    if (chunk < 128) chunk = 128;
-    p.chunk = (int)chunk;
-    p.splits = (int)((vis + chunk - 1) / chunk);
+    // Splits: blocks run two a multiprocessor, a unit's splits one grid row after the other, so
+    // that the last, shorter ones fill up what the others leave. The time of a chunk size, in
+    // keys of streaming: the work over the slots and a last block, at least one block; `start`
+    // is what a block's start and join take. Candidates fill one to six waves, evenly or
+    // with a short last split.
+    const long long slots = 2 * kPlanSms, start = 16384 / d;
+    long long best = -1;
+    p.chunk = 128;
+    p.splits = 0;
+    for (int i = 0; i < 20 && vis > 0; ++i) {
+        const int k = i / 2;
+        const long long want = k < 4 ? k + 1 : (k - 3) * slots / units;
+        if (want < 1) continue;
+        long long chunk = (vis + want - 1) / want;
+        if (i & 1) chunk += chunk / 4;
+        chunk = (chunk + 127) / 128 * 128;
+        const long long n = (vis + chunk - 1) / chunk, last = vis - (n - 1) * chunk;
+        const long long cost = n * units <= slots ? slots * ((n > 1 ? chunk : vis) + start)
+                                                  : units * (vis + n * start) + slots * (last + start);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p.chunk = (int)chunk;
+            p.splits = (int)n;
+        }
+    }
     p.p_splits = p.p_tiles = 0;
     if (P > 0) {
         const long long per = 128 / q_rows;
         const long long tiles = per ? (B + per - 1) / per : B * ((q_rows + 127) / 128);
         const long long u = (tiles + 1) / 2 * Hkv;
         const int nk = (P + 127) / 128;
-        long long best = -1;
+        best = -1;
         for (int n = 1; n <= nk && n <= 2 * kPlanSms; ++n) {
             const int s = (nk + n - 1) / n, real = (nk + s - 1) / s;
             // Waves of blocks times their steps; two steps' time to fill and drain a block.
@@ -581,7 +607,7 @@ int decode_step(const StepArgs& a) {
     c.rows = plan.rows;
     auto kernel = a.d == 64 ? (f16 ? bfk::dec::combine_kernel<64, true> : bfk::dec::combine_kernel<64, false>)
                             : (f16 ? bfk::dec::combine_kernel<128, true> : bfk::dec::combine_kernel<128, false>);
-    return launch_error(launch_pdl(kernel, dim3((unsigned)plan.rows), 128, 0, a.stream, c));
+    return launch_error(launch_pdl(kernel, dim3((unsigned)plan.rows), bfk::dec::kJoinWarps * 32, 0, a.stream, c));
 }
 
 }  // namespace

@@ -59,46 +59,52 @@ struct __align__(sizeof(T) * V) Vec {
 };
 
 constexpr int kBlock = 256;
-constexpr int kMaxTile = 8;      // tokens of a block
+constexpr int kMaxTile = 4;      // tokens of a block: 72 us at B=4 N=4095 Hq=32 Hk=8 d=128 (a copy: 58), 8: 74, 2: 75
 constexpr int kMaxPairs = 512;  // (token, pair) entries of a block's table
 
 // A work item is V consecutive columns of one row: of the first half with their partners of
-// the second half (half layout), of the rotated part (interleaved), or copied columns.
+// the second half (half layout), of the rotated part (interleaved), or copied columns. A thread
+// keeps its item and steps through the rows (token, head) of its block. Few registers and a
+// full multiprocessor of threads (2048) carry more bytes in flight than more loads a thread do.
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kBlock) rotary_kernel(const Params p) {
+__global__ void __launch_bounds__(kBlock, 8) rotary_kernel(const Params p) {
     __shared__ float2 cs[kMaxPairs];
-    __shared__ int tok_b[kMaxTile], tok_n[kMaxTile];
+    __shared__ const char* x_at[2][kMaxTile];  // a token's row of head 0
+    __shared__ char* y_at[2][kMaxTile];
+    __shared__ long long pos_at[kMaxTile];
     const int half = p.rot / 2;
     const long long t0 = (long long)blockIdx.x * p.tile;
     const int nt = (int)min((long long)p.tile, p.tokens - t0);
     griddep_launch_dependents();
     griddep_wait();
     if (threadIdx.x < nt) {
-        const long long tok = t0 + threadIdx.x, b = tok / p.n;
-        tok_b[threadIdx.x] = (int)b;
-        tok_n[threadIdx.x] = (int)(tok - b * p.n);
+        const long long tok = t0 + threadIdx.x, b = tok / p.n, n = tok - b * p.n;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            x_at[w][threadIdx.x] = p.x[w] + b * p.xs[w][0] + n * p.xs[w][2];
+            y_at[w][threadIdx.x] = p.y[w] + (b * p.heads[w] * p.n + n) * p.d * (int)sizeof(T);
+        }
+        pos_at[threadIdx.x] = b * p.pos_stride + n;
     }
     __syncthreads();
+
     for (int i = threadIdx.x; i < nt * half; i += kBlock) {
-        const int t = i / half, pr = i - t * half;
-        const long long at = tok_b[t] * p.pos_stride + tok_n[t];
+        const int tt = i / half, pr = i - tt * half;
+        const long long at = pos_at[tt];
         const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
                                       : (long long)reinterpret_cast<const int*>(p.positions)[at];
         const double turns = (double)pos * (p.freqs[pr] * 0.15915494309189533577);
         const double angle = 2.0 * (turns - rint(turns));  // in units of pi, [-1, 1]
         const float hi = (float)angle;
-        float s, c;
-        sincospif(hi, &s, &c);
+        float s, co;
+        sincospif(hi, &s, &co);
         // First-order step for what the cast to fp32 dropped (up to 2^-24 of the angle).
         const float lo = (float)(angle - (double)hi) * 3.14159265f;
-        cs[i] = make_float2((c - s * lo) * p.amplitude, (s + c * lo) * p.amplitude * p.sign);
+        cs[i] = make_float2((co - s * lo) * p.amplitude, (s + co * lo) * p.amplitude * p.sign);
     }
     __syncthreads();
 
-    // Items of a row: the rotated ones, then the copied ones. A thread keeps its item and steps
-    // through the rows (token, head) of the block, kAhead of them at a time with all loads
-    // before the first product, so that enough bytes are in flight.
-    const int rot_items = kInterleaved ? p.rot / V : half / V;
+    const int rot_items = kInterleaved ? p.rot / V : half / V;  // of a row; then the copied ones
     const int row_items = rot_items + (p.d - p.rot) / V;
     const int all_heads = p.heads[0] + p.heads[1];
     const int h0 = (int)((long long)all_heads * blockIdx.y / p.head_split);
@@ -107,60 +113,43 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(const Params p) {
     const int first = threadIdx.x / across;
     if (first >= pass) return;
     using VT = Vec<T, V>;
-    constexpr int kAhead = 4;
+    const long long y_head = (long long)p.n * p.d * (int)sizeof(T);
     for (int item = threadIdx.x - first * across; item < row_items; item += kBlock) {
         const bool turned = item < rot_items;
         const int col = turned ? item * V : p.rot + (item - rot_items) * V;
-        const int pair = kInterleaved ? col >> 1 : col;
         int t = first / nh, h = first - t * nh;
         while (t < nt) {
-            VT a[kAhead], c[kAhead];
-            T* dst[kAhead];
-            const float2* tab[kAhead];
-            int live = 0;
+            const int hh = h0 + h, w = hh >= p.heads[0], hw = w ? hh - p.heads[0] : hh;
+            const T* x = reinterpret_cast<const T*>(x_at[w][t] + hw * p.xs[w][1]) + col;
+            T* y = reinterpret_cast<T*>(y_at[w][t] + hw * y_head) + col;
+            VT a = *reinterpret_cast<const VT*>(x);
+            if (turned) {
+                const float2* tab = cs + t * half + (kInterleaved ? col >> 1 : col);
+                if constexpr (kInterleaved) {
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (t < nt) {
-                    const int hh = h0 + h, which = hh >= p.heads[0], hw = which ? hh - p.heads[0] : hh;
-                    const long long b = tok_b[t], n = tok_n[t];
-                    const T* x = reinterpret_cast<const T*>(p.x[which] + b * p.xs[which][0] + hw * p.xs[which][1] +
-                                                            n * p.xs[which][2]) + col;
-                    dst[k] = reinterpret_cast<T*>(p.y[which]) + ((b * p.heads[which] + hw) * p.n + n) * p.d + col;
-                    tab[k] = cs + t * half + pair;
-                    a[k] = *reinterpret_cast<const VT*>(x);
-                    if (!kInterleaved && turned) c[k] = *reinterpret_cast<const VT*>(x + half);
-                    live = k + 1;
-                    h += pass;
-                    while (h >= nh) {
-                        h -= nh;
-                        ++t;
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 cw = tab[e >> 1];
+                        const float u = to_f<T>(a.e[e]), v = to_f<T>(a.e[e + 1]);
+                        a.e[e] = from_f<T>(u * cw.x - v * cw.y);
+                        a.e[e + 1] = from_f<T>(u * cw.y + v * cw.x);
                     }
+                } else {
+                    VT c = *reinterpret_cast<const VT*>(x + half);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float2 cw = tab[e];
+                        const float u = to_f<T>(a.e[e]), v = to_f<T>(c.e[e]);
+                        a.e[e] = from_f<T>(u * cw.x - v * cw.y);
+                        c.e[e] = from_f<T>(u * cw.y + v * cw.x);
+                    }
+                    *reinterpret_cast<VT*>(y + half) = c;
                 }
             }
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (k >= live) break;
-                if (turned) {
-                    if constexpr (kInterleaved) {
-#pragma unroll
-                        for (int e = 0; e < V; e += 2) {
-                            const float2 w = tab[k][e >> 1];
-                            const float u = to_f<T>(a[k].e[e]), v = to_f<T>(a[k].e[e + 1]);
-                            a[k].e[e] = from_f<T>(u * w.x - v * w.y);
-                            a[k].e[e + 1] = from_f<T>(u * w.y + v * w.x);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float2 w = tab[k][e];
-                            const float u = to_f<T>(a[k].e[e]), v = to_f<T>(c[k].e[e]);
-                            a[k].e[e] = from_f<T>(u * w.x - v * w.y);
-                            c[k].e[e] = from_f<T>(u * w.y + v * w.x);
-                        }
-                        *reinterpret_cast<VT*>(dst[k] + half) = c[k];
-                    }
-                }
-                *reinterpret_cast<VT*>(dst[k]) = a[k];
+            *reinterpret_cast<VT*>(y) = a;
+            h += pass;
+            while (h >= nh) {
+                h -= nh;
+                ++t;
             }
         }
     }
