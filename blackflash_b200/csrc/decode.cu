@@ -347,8 +347,62 @@ struct CombineParams {
     long long rows;
 };
 
+// Up to 32 parts: one warp per row, lane i with part i's weight, no barrier.
+template <int D, bool kF16>
+__global__ void __launch_bounds__(128) combine_few_kernel(const CombineParams p) {
+    griddep_wait();
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const int lane = threadIdx.x & 31;
+    constexpr int E = D / 32;
+    const int total = p.n[0] + p.n[1];
+    float x = -INFINITY;
+    if (lane < p.n[0])
+        x = p.lse[0][(size_t)lane * p.rows + row];
+    else if (lane < total)
+        x = p.lse[1][(size_t)(lane - p.n[0]) * p.rows + row];
+    float m = x;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    const float mine = x == -INFINITY ? 0.f : fast_exp2(x - m);
+    float y[E], l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = 0.f;
+    constexpr int kBatch = 8;  // loads in flight
+    for (int i0 = 0; i0 < total; i0 += kBatch) {
+        float a[kBatch][E];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = min(i0 + k, total - 1);
+            const float* src = (i < p.n[0] ? p.o[0] + ((size_t)i * p.rows + row) * D
+                                           : p.o[1] + ((size_t)(i - p.n[0]) * p.rows + row) * D) + lane * E;
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                a[k][0] = v.x, a[k][1] = v.y, a[k][2] = v.z, a[k][3] = v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(src);
+                a[k][0] = v.x, a[k][1] = v.y;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float w = i0 + k < total ? __shfl_sync(0xffffffffu, mine, (i0 + k) & 31) : 0.f;
+            l += w;
+            // Weight 0: no visible key (that output was not written), or nothing beside the largest.
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] += w == 0.f ? 0.f : w * a[k][e];
+        }
+    }
+    const bool any = l > 0.f || l != l;  // NaN stays NaN
+    const float inv = any ? 1.f / l : 0.f;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out) + row * (D / 2) + lane * (E / 2);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) out[e] = pack2<kF16>(y[2 * e] * inv, y[2 * e + 1] * inv);
+    if (lane == 0 && p.lse_out) p.lse_out[row] = any ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
 // One block per row, one warp per share of its parts: O = sum_i w_i O_i / sum_i w_i with
-// w_i = 2^(lse_i - max). Parts without a visible key (-inf) are not read.
+// w_i = 2^(lse_i - max). Parts without a visible key (-inf) weigh nothing, whatever their output holds.
 constexpr int kJoinWarps = 8;
 template <int D, bool kF16>
 __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const CombineParams p) {
@@ -372,24 +426,31 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const CombineP
     float y[E], l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] = 0.f;
-#pragma unroll 8
-    for (int i = warp; i < total; i += kJoinWarps) {
-        const float x = lse_at(i);
-        if (x == -INFINITY) continue;
-        const float w = fast_exp2(x - m);
-        const float* src = (i < p.n[0] ? p.o[0] + ((size_t)i * p.rows + row) * D
-                                       : p.o[1] + ((size_t)(i - p.n[0]) * p.rows + row) * D) + lane * E;
-        l += w;
-        float a[E];
-        if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src);
-            a[0] = v.x, a[1] = v.y, a[2] = v.z, a[3] = v.w;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(src);
-            a[0] = v.x, a[1] = v.y;
+    constexpr int kBatch = 4;  // loads in flight
+    for (int i0 = warp; i0 < total; i0 += kJoinWarps * kBatch) {
+        float a[kBatch][E], x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int j = i0 + k * kJoinWarps, i = min(j, total - 1);
+            x[k] = j < total ? lse_at(i) : -INFINITY;
+            const float* src = (i < p.n[0] ? p.o[0] + ((size_t)i * p.rows + row) * D
+                                           : p.o[1] + ((size_t)(i - p.n[0]) * p.rows + row) * D) + lane * E;
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                a[k][0] = v.x, a[k][1] = v.y, a[k][2] = v.z, a[k][3] = v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(src);
+                a[k][0] = v.x, a[k][1] = v.y;
+            }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] += w * a[e];
+        for (int k = 0; k < kBatch; ++k) {
+            const float w = x[k] == -INFINITY ? 0.f : fast_exp2(x[k] - m);
+            l += w;
+            // Weight 0: no visible key (that output was not written), or nothing beside the largest.
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] += w == 0.f ? 0.f : w * a[k][e];
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sm_y[warp][lane * E + e] = y[e];
@@ -526,7 +587,7 @@ int decode_step(const StepArgs& a) {
     if (!a.q || !a.o || ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u))
         return bf_set_error(BF_ERR_ARG, "Q and O must be non-null and 16-byte aligned");
     if (a.C > 0 && !a.lengths) return bf_set_error(BF_ERR_ARG, "lengths: null pointer");
-    if (plan.bytes > 0 && (!a.ws || a.ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a.ws) & 15u)))
+    if (plan.bytes > 0 && (!a.ws || a.ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a.ws) & 31u)))
         return bf_set_error(BF_ERR_ARG, "workspace null, misaligned or smaller than blackflash_decode_workspace_bytes()");
     const bool f16 = a.dtype == BF_DTYPE_F16;
     float* part_o = reinterpret_cast<float*>(a.ws);
@@ -605,6 +666,13 @@ int decode_step(const StepArgs& a) {
     c.out = a.o;
     c.lse_out = a.lse;
     c.rows = plan.rows;
+    // A block per row where there are more parts than lanes: 128 parts of 32 rows took 9 us by
+    // one warp a row; 18 parts of 2048 rows take 10.5 us by a block a row, 4 by a warp.
+    if (plan.splits + plan.p_splits <= 32) {
+        auto kernel = a.d == 64 ? (f16 ? bfk::dec::combine_few_kernel<64, true> : bfk::dec::combine_few_kernel<64, false>)
+                                : (f16 ? bfk::dec::combine_few_kernel<128, true> : bfk::dec::combine_few_kernel<128, false>);
+        return launch_error(launch_pdl(kernel, dim3((unsigned)((plan.rows + 3) / 4)), 128, 0, a.stream, c));
+    }
     auto kernel = a.d == 64 ? (f16 ? bfk::dec::combine_kernel<64, true> : bfk::dec::combine_kernel<64, false>)
                             : (f16 ? bfk::dec::combine_kernel<128, true> : bfk::dec::combine_kernel<128, false>);
     return launch_error(launch_pdl(kernel, dim3((unsigned)plan.rows), bfk::dec::kJoinWarps * 32, 0, a.stream, c));

@@ -444,22 +444,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int col = h * (D / 2) + 32 * part;
                 const float f = kDQ || which ? p.scale : 1.f;
                 if (it.slot >= 0) {
-                    float4* dst = reinterpret_cast<float4*>(p.part + ((it.slot * 2 + which) * 128 + row) * D + col);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        dst[c] = make_float4(__uint_as_float(o[4 * c]) * f, __uint_as_float(o[4 * c + 1]) * f,
-                                             __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
-                } else if (xrow < (kDQ ? p.n_q : p.n_kv)) {
-                    __nv_bfloat16* base = kDQ ? p.dq + (((size_t)it.b * p.hq + it.head) * p.n_q + xrow) * D
-                                              : (which ? p.dk : p.dv) + (((size_t)it.b * p.hkv + it.kvh) * p.n_kv + xrow) * D;
-                    uint4* dst = reinterpret_cast<uint4*>(base + col);
+                    float* dst = p.part + ((it.slot * 2 + which) * 128 + row) * D + col;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t w[4];
+                        uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * e]) * f, __uint_as_float(o[8 * c + 2 * e + 1]) * f);
-                        dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(__uint_as_float(o[8 * c + e]) * f);
+                        st_global_v8(dst + 8 * c, w);
+                    }
+                } else if (xrow < (kDQ ? p.n_q : p.n_kv)) {
+                    __nv_bfloat16* dst = (kDQ ? p.dq + (((size_t)it.b * p.hq + it.head) * p.n_q + xrow) * D
+                                              : (which ? p.dk : p.dv) + (((size_t)it.b * p.hkv + it.kvh) * p.n_kv + xrow) * D) +
+                                         col;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w[e] = pack_bf16x2(__uint_as_float(o[16 * c + 2 * e]) * f, __uint_as_float(o[16 * c + 2 * e + 1]) * f);
+                        st_global_v8(dst + 16 * c, w);
                     }
                 }
             }

@@ -432,23 +432,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (row_ok) {
                     const size_t at = idx * D + h * (D / 2) + part * 32;
                     if constexpr (kPartial) {
-                        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            dst[c] = make_float4(__uint_as_float(o[4 * c]) * inv, __uint_as_float(o[4 * c + 1]) * inv,
-                                                 __uint_as_float(o[4 * c + 2]) * inv, __uint_as_float(o[4 * c + 3]) * inv);
-                    } else {
-                        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + at);
+                        float* dst = reinterpret_cast<float*>(p.out) + at;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            uint32_t w[4];
+                            uint32_t w[8];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float a = __uint_as_float(o[8 * c + 2 * e]) * inv;
-                                const float b = __uint_as_float(o[8 * c + 2 * e + 1]) * inv;
+                            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(__uint_as_float(o[8 * c + e]) * inv);
+                            st_global_v8(dst + 8 * c, w);
+                        }
+                    } else {
+                        uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + at;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float a = __uint_as_float(o[16 * c + 2 * e]) * inv;
+                                const float b = __uint_as_float(o[16 * c + 2 * e + 1]) * inv;
                                 w[e] = kF16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
                             }
-                            dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                            st_global_v8(dst + 16 * c, w);
                         }
                     }
                 }

@@ -74,7 +74,7 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
     if ((rc = check_view(Q, "Q", B, Hq, Nq, d, 2, &sq)) != BF_OK) return rc;
     if ((rc = check_view(K, "K", B, Hkv, Nkv, d, 2, &sk)) != BF_OK) return rc;
     if ((rc = check_view(V, "V", B, Hkv, Nkv, d, 2, &sv)) != BF_OK) return rc;
-    if (!O || (reinterpret_cast<uintptr_t>(O) & 15u)) return bf_set_error(BF_ERR_ARG, "O must be 16-byte aligned");
+    if (!O || (reinterpret_cast<uintptr_t>(O) & 31u)) return bf_set_error(BF_ERR_ARG, "O must be 32-byte aligned");
 
     bfk::win::Params p;
     memset(&p, 0, sizeof(p));
@@ -189,8 +189,8 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     if ((rc = check_view(dO, "dO", B, Hq, Nq, d, 2, &sd)) != BF_OK) return rc;
     const void* ptrs[] = {O, dQ, dK, dV, workspace};
     for (const void* ptr : ptrs)
-        if (!ptr || (reinterpret_cast<uintptr_t>(ptr) & 15u))
-            return bf_set_error(BF_ERR_ARG, "O, dQ, dK, dV and the workspace must be non-null and 16-byte aligned");
+        if (!ptr || (reinterpret_cast<uintptr_t>(ptr) & 31u))
+            return bf_set_error(BF_ERR_ARG, "O, dQ, dK, dV and the workspace must be non-null and 32-byte aligned");
     if (!lse) return bf_set_error(BF_ERR_ARG, "lse: null pointer");
     const BwdPlan plan = bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks);
     if (workspace_bytes < plan.bytes)

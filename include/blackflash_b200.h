@@ -170,7 +170,8 @@ typedef struct {
  * Causal attention with a sliding window and sinks, grouped KV heads. No counterpart in the
  * reference.
  *   Q: [B, Hq, Nq, d], K, V: [B, Hkv, Nkv, d], bf16 or fp16, d = 64 or 128, Hq a multiple
- *   of Hkv; query head h reads KV head h / (Hq / Hkv). O: [B, Hq, Nq, d] contiguous.
+ *   of Hkv; query head h reads KV head h / (Hq / Hkv). O: [B, Hq, Nq, d] contiguous, 32-byte
+ *   aligned.
  *   lse: [B, Hq, Nq] fp32 natural logsumexp, optional.
  * Query i stands at position p = i + Nkv - Nq (the last query at the last key) and sees the
  * keys j <= p with j > p - window or j < sinks. window >= Nkv is plain causal attention. A
@@ -187,7 +188,8 @@ int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const bf_view* V, 
  * contiguous, summed over the query heads that share a KV head. Rows that see nothing, and
  * keys that nothing sees, get zeros. The result does not depend on scheduling: no atomics.
  *   workspace: device memory of blackflash_window_bwd_workspace_bytes(...) bytes (-1 for bad
- *   sizes), 16-byte aligned, overwritten. Calls that overlap on the GPU need their own.
+ *   sizes), overwritten. Calls that overlap on the GPU need their own. O, the gradients and the
+ *   workspace are 32-byte aligned.
  */
 long long blackflash_window_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks);
 int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, const void* O, const bf_view* dO,
@@ -209,7 +211,7 @@ int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, 
  * never read.
  *   workspace: device memory of blackflash_decode_workspace_bytes(...) bytes (P = 0 for
  *   blackflash_window_decode; window = INT_MAX and sinks = 0 for blackflash_prefix_decode),
- *   16-byte aligned, overwritten; null where that is 0. It returns -1 for bad sizes. Calls
+ *   32-byte aligned, overwritten; null where that is 0. It returns -1 for bad sizes. Calls
  *   that overlap on the GPU need workspaces of their own.
  */
 long long blackflash_decode_workspace_bytes(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, int sinks);

@@ -36,9 +36,9 @@ def test_window_backward_plans(lib, change):
 def test_window_backward_refusals(lib):
     ok, sizes = view(lib), (1, 2, 2, 8, 8, 64, 4, 0, 0.125, None)
     need = lib.blackflash_window_bwd_workspace_bytes(*sizes[:8])
-    good = [ok, ok, ok, 16, ok, 16, 16, 16, 16, 16, need]
+    good = [ok, ok, ok, 32, ok, 16, 32, 32, 32, 32, need]
     for i, bad, text in ((0, None, b"Q:"), (4, view(lib, strides=(64, 3, 64)), b"dO"), (3, None, b"O, dQ"), (5, None, b"lse"),
-                         (8, 24, b"O, dQ"), (9, None, b"workspace"), (10, need - 1, b"workspace")):
+                         (8, 16, b"O, dQ"), (9, None, b"workspace"), (10, need - 1, b"workspace")):
         args = list(good)
         args[i] = bad
         assert lib.blackflash_window_bwd(*args, *sizes) == 1 and text in lib.blackflash_last_error()
@@ -57,7 +57,7 @@ WINDOW = dict(B=1, Hq=2, Hkv=1, Nq=8, Nkv=8, d=64, window=4, sinks=0, scale=0.12
 def test_window_fwd_refuses_sizes(lib, change, text):
     a = {**WINDOW, **change}
     v = view(lib, strides=(1 << 20, 1 << 14, 64))
-    rc = lib.blackflash_window_fwd(v, v, v, 16, None, *(a[x] for x in WINDOW), None)
+    rc = lib.blackflash_window_fwd(v, v, v, 32, None, *(a[x] for x in WINDOW), None)
     assert rc == 1 and text in lib.blackflash_last_error(), lib.blackflash_last_error()
 
 
@@ -70,9 +70,9 @@ def test_views_are_checked(lib, bad, text):
     for i in range(3):
         views = [ok, ok, ok]
         views[i] = view(lib, **bad)
-        rc = lib.blackflash_window_fwd(*views, 16, None, *{**WINDOW, "Hkv": 2}.values(), None)
+        rc = lib.blackflash_window_fwd(*views, 32, None, *{**WINDOW, "Hkv": 2}.values(), None)
         assert rc == 1 and text in lib.blackflash_last_error()
-    rc = lib.blackflash_window_fwd(ok, ok, ok, 8, None, *WINDOW.values(), None)
+    rc = lib.blackflash_window_fwd(ok, ok, ok, 16, None, *WINDOW.values(), None)
     assert rc == 1 and b"O must" in lib.blackflash_last_error()
 
 
@@ -91,14 +91,14 @@ def test_decode_plans_and_refusals(lib):
     v = view(lib)
     need = ws(1, 8, 2, 1, 0, 100000, 64, 5000, 4)
     sizes = (1, 8, 2, 1, 100000, 64, 5000, 4, 0.125, 0, None)
-    for args, text in (((None, v, v, 16, 16, None, 16, need), b"Q and O"), ((16, v, v, None, 16, None, 16, need), b"lengths"),
-                       ((16, v, v, 16, 16, None, 16, need - 1), b"workspace"), ((16, v, v, 16, 16, None, None, need), b"workspace"),
-                       ((16, v, v, 16, 16, None, 24, need), b"workspace"), ((16, None, v, 16, 16, None, 16, need), b"K_cache")):
+    for args, text in (((None, v, v, 16, 16, None, 16, need), b"Q and O"), ((16, v, v, None, 16, None, 32, need), b"lengths"),
+                       ((16, v, v, 16, 16, None, 32, need - 1), b"workspace"), ((16, v, v, 16, 16, None, None, need), b"workspace"),
+                       ((16, v, v, 16, 16, None, 16, need), b"workspace"), ((16, None, v, 16, 16, None, 32, need), b"K_cache")):
         assert lib.blackflash_window_decode(*args, *sizes) == 1
         assert text in lib.blackflash_last_error()
     big = 1 << 30
     p = (1, 8, 2, 1, 100, 50, 64)
-    for args, text in (((16, None, v, v, v, 16, 16, None, 16, big), b"prefix"), ((16, v, v, v, None, 16, 16, None, 16, big), b"V_cache"),
+    for args, text in (((16, None, v, v, v, 16, 16, None, 32, big), b"prefix"), ((16, v, v, v, None, 16, 16, None, 32, big), b"V_cache"),
                        ((16, v, v, v, v, 16, 16, None, None, big), b"workspace")):
         assert lib.blackflash_prefix_decode(*args, *p, 0.125, 0, None) == 1
         assert text in lib.blackflash_last_error()
