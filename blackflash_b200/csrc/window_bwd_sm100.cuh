@@ -338,9 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int c = 0; c < NC; ++c) pr[c] = __uint_as_float(s[c]);
                 }
                 if (last < NC || (first > 0 && snk < NC)) {
+                    const uint32_t see = win::below(last) & (~win::below(first) | win::below(snk));  // a bit per column
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
-                        if (c >= last || (c < first && c >= snk)) pr[c] = -INFINITY;
+                        if (!(see & (1u << c))) pr[c] = -INFINITY;
                 }
 #pragma unroll
                 for (int c = 0; c < NC; c += 2) {

@@ -174,6 +174,11 @@ __device__ __forceinline__ void decode(const Params& p, int item, Item& it) {
     }
 }
 
+// Bits 0 .. n - 1 (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t below(int n) {
+    return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u;
+}
+
 // a[t] for the two-entry arrays of an Item, which stay in registers.
 template <typename T>
 __device__ __forceinline__ T pick(const T (&a)[2], int t) {
@@ -293,22 +298,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(bar_se);  // S_t is in registers
 
                 const int c0 = j * 128 + h * 64;
-                if constexpr (kPartial) {
-                    const int valid = p.n_kv - c0;
-                    if (valid < 64) {
+                // Seen: column c with c < last, and c >= first or c < snk. As a word of bits per 32
+                // columns a column costs two instructions, not the four of the comparisons (which
+                // took as long as the exponentials: two or three steps of an item are masked).
+                const int last = kPartial ? p.n_kv - c0 : pos + 1 - c0;
+                const int first = kPartial ? 0 : pos + 1 - p.window - c0;
+                const int snk = kPartial ? 0 : p.sinks - c0;
+                if (last < 64 || (first > 0 && snk < 64)) {
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c >= valid) s[c >> 5][c & 31] = __float_as_uint(-INFINITY);
-                    }
-                } else {
-                    // Seen: column c with c < last, and c >= first or c < snk.
-                    const int last = pos + 1 - c0;
-                    const int first = pos + 1 - p.window - c0;
-                    const int snk = p.sinks - c0;
-                    if (last < 64 || (first > 0 && snk < 64)) {
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t see = below(last - 32 * q) & (~below(first - 32 * q) | below(snk - 32 * q));
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c >= last || (c < first && c >= snk)) s[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see & (1u << c))) s[q][c] = __float_as_uint(-INFINITY);
                     }
                 }
 
