@@ -15,6 +15,8 @@
 //     its own. With an even group the two are two heads at the same rows, so both lists
 //     are the same and K/V are read once for both; otherwise they are two consecutive row
 //     blocks, and a tile sits out the steps that only the other one needs;
+//   * up to 32 sinks (kNarrow) the step of the sink tile is 32 columns wide: it comes
+//     first, so it has no maximum to compare with and nothing to rescale;
 //   * the list is the sink tiles [0, ns) and then the window's tiles [lo, hi), so the work
 //     of a row is proportional to the keys that it sees and not to the length;
 //   * a tile may be wholly masked for some of its rows (the window's lower edge, rows
@@ -90,6 +92,18 @@ enum : unsigned {
     kSiteSoftPV = 0x741,
 };
 
+// n / d by a product, for 0 <= n < 2^31 and d >= 1: with l = ceil(log2 d) and
+// m = floor(2^32 (2^l - d) / d) + 1, n / d = (floor(m n / 2^32) + n) >> l (Granlund and
+// Montgomery 1994).
+struct FastDiv {
+    uint32_t m, l;
+    void set(uint32_t d) {
+        for (l = 0; (1ull << l) < d; ++l) {}
+        m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
+};
+
 struct Params {
     int items;
     int batch, hq, hkv, group;
@@ -101,6 +115,7 @@ struct Params {
     unsigned long long timeout_ns;
     // window mode
     int window, sinks, ns;  // window clamped to n_kv, sinks, sink tiles
+    FastDiv by_units, by_heads, by_group;
     int q_blocks;           // item blocks along the queries
     int pair_heads;         // the two tiles are two heads of a group
     // partial mode
@@ -146,12 +161,12 @@ __device__ __forceinline__ void decode(const Params& p, int item, Item& it) {
         const int per_head = p.pair_heads ? p.hq / 2 : p.hq;
         const int units = p.batch * per_head;
         // Late rows see the most keys: they are handed out first.
-        const int qb = p.q_blocks - 1 - item / units;
-        const int unit = item % units;
-        const int b = unit / per_head, hu = unit % per_head;
+        const int late = p.by_units(item), unit = item - late * units;
+        const int qb = p.q_blocks - 1 - late;
+        const int b = p.by_heads(unit), hu = unit - b * per_head;
         it.split = 0;
         it.kvb = b;
-        it.kvh = (p.pair_heads ? 2 * hu : hu) / p.group;
+        it.kvh = p.by_group(p.pair_heads ? 2 * hu : hu);
         const int off = p.n_kv - p.n_q;
         int lo_u = p.nk, hi_u = 0;
 #pragma unroll
@@ -189,7 +204,7 @@ __device__ __forceinline__ bool sees(const Params& p, const Item& it, int t, int
     return j < pick(it.hi, t) && (j >= pick(it.lo, t) || j < p.ns);
 }
 
-template <int D, bool kF16, bool kPartial>
+template <int D, bool kF16, bool kPartial, bool kNarrow>
 __global__ void __launch_bounds__(kThreads, 1)
     window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const Params p) {
@@ -285,7 +300,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m_use = -INFINITY;  // log2-domain maximum that P, O and l refer to
             float l_half = 0.f;       // row sum over this thread's column half
 
-            for (int s_i = 0; s_i < steps; ++s_i, ++g) {
+            if (kNarrow && n_sink > 0 && steps > 0) {
+                // The sinks' step, 32 columns: this thread's are 16 h .. 16 h + 15. Every row of the
+                // tile is past the sinks (lo > 0) and sees them all.
+                if (!(ok = warp_wait(bar_s, g & 1u, ctl, kSiteSoftS))) break;
+                tc_fence_after();
+                uint32_t s[16], pk[8];
+                tmem_ld16x32bx2_x16<16>(tS, s);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_se);
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    if (c >= p.sinks - h * 16) s[c] = __float_as_uint(-INFINITY);
+                    mx = fmaxf(mx, __uint_as_float(s[c]));
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                m_use = mx * p.scale_log2;
+                const float neg_m = m_use == -INFINITY ? 0.f : kShift - m_use;
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                    const float p0 = fast_exp2(fmaf(__uint_as_float(s[c]), p.scale_log2, neg_m));
+                    const float p1 = fast_exp2(fmaf(__uint_as_float(s[c + 1]), p.scale_log2, neg_m));
+                    l_half += p0 + p1;
+                    pk[c / 2] = kF16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+                }
+                if (C::kSepP && g > 0) {
+                    if (!(ok = warp_wait(bar_pv, (g - 1) & 1u, ctl, kSiteSoftPV))) break;
+                    tc_fence_after();
+                }
+                tmem_st16x32bx2_x8<8>(tP, pk);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p);
+                ++g;
+            }
+            for (int s_i = kNarrow ? n_sink : 0; s_i < steps; ++s_i, ++g) {
                 const int j = s_i < n_sink ? s_i : s_i + skip;
                 if (!(ok = warp_wait(bar_s, g & 1u, ctl, kSiteSoftS))) break;
                 tc_fence_after();
@@ -542,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kFmt = kF16 ? ~((1u << 7) | (1u << 10)) : ~0u;  // A and B format bits: 0 = fp16, 1 = bf16
         constexpr uint32_t kIdescS = idesc_bf16_f32(128, 128, 0) & kFmt;
         constexpr uint32_t kIdescSh = idesc_bf16_f32(128, 64, 0) & kFmt;
+        constexpr uint32_t kIdescSn = idesc_bf16_f32(128, 32, 0) & kFmt;
         constexpr uint32_t kHalfRowsLo = (64 * 128) >> 4;  // K rows 64.. inside a chunk
         constexpr uint32_t kIdescO = idesc_bf16_f32(128, 64, 1) & kFmt;
         constexpr uint32_t kChunkLo = C::kChunkBytes >> 4;
@@ -575,10 +629,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t k_lo = lo0 + (C::kOffK >> 4) + st * kTileLo;
                         const uint32_t q_lo = lo0 + (C::kOffQ >> 4) + (uint32_t)(qb * 2 + ts) * kTileLo;
                         const uint32_t d = tmem + ts * 128;
+                        const bool narrow = kNarrow && j < pick(it.lo, ts);
                         if (g[0] > 0 && !(ok = warp_wait(smem_addr(&bars->s_empty[ts]), (g[0] - 1) & 1u, ctl, kSiteMmaK + 3 + ts)))
                             break;
                         tc_fence_after();
-                        if constexpr (C::kSepP) {
+                        if (narrow) {  // keys 0..31 alone
+                            if (!C::kSepP && g[0] > 0 &&
+                                !(ok = warp_wait(smem_addr(&bars->pv_done[ts]), (g[0] - 1) & 1u, ctl, kSiteMmaK + 1 + ts)))
+                                break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t off = (uint32_t)(kk >> 2) * kChunkLo + (uint32_t)(kk & 3) * 2;
+                                umma_ss_on(on, d, q_lo + off, k_lo + off, desc_hi, kIdescSn, kk > 0);
+                            }
+                        } else if constexpr (C::kSepP) {
 #pragma unroll
                             for (int kk = 0; kk < D / 16; ++kk)
                                 umma_ss_on(on, d, q_lo + kk * 2, k_lo + kk * 2, desc_hi, kIdescS, kk > 0);
@@ -614,11 +679,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!sees(p, it, t, j)) continue;
                         if (!(ok = warp_wait(smem_addr(&bars->p_full[t]), g[t] & 1u, ctl, kSiteMmaV + 1 + t))) break;
                         tc_fence_after();
+                        const uint32_t rest = kNarrow && j < it.lo[t] ? 0u : on;  // past key 31
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)  // 16 keys: 8 TMEM columns of P, 16 x 128 bytes of V
 #pragma unroll
                             for (int ch = 0; ch < C::kChunks; ++ch)
-                                umma_ts_on(on, tmem + C::kColO + t * D + ch * 64, tmem + C::kColP + t * C::kStepP + kk * 8,
+                                umma_ts_on(kk < 2 ? on : rest, tmem + C::kColO + t * D + ch * 64, tmem + C::kColP + t * C::kStepP + kk * 8,
                                            v_lo + ch * kChunkLo + kk * 128, desc_hi, kIdescO, !first[t] || kk > 0);
                         umma_commit_on(on, smem_addr(&bars->pv_done[t]));
                         first[t] = false;

@@ -27,11 +27,11 @@ namespace {
 constexpr unsigned long long kTimeoutNs = 4000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, bool kF16, bool kPartial>
+template <int D, bool kF16, bool kPartial, bool kNarrow>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const bfk::win::Params& p,
                cudaStream_t stream) {
     static std::atomic<bool> done[64];  // per device; zero-initialised (static storage)
-    auto kernel = bfk::win::window_fwd_kernel<D, kF16, kPartial>;
+    auto kernel = bfk::win::window_fwd_kernel<D, kF16, kPartial, kNarrow>;
     int rc, sms = 0;
     if ((rc = allow_smem(kernel, bfk::win::smem_bytes<D>(), done)) != BF_OK) return rc;
     if ((rc = sm_count(&sms)) != BF_OK) return rc;
@@ -40,14 +40,14 @@ int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
                                    mk, mv, p));
 }
 
-template <bool kPartial>
+template <bool kPartial, bool kNarrow>
 int launch_fwd(int d, bool f16, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                const bfk::win::Params& p, cudaStream_t stream) {
     if (d == 64)
-        return f16 ? launch_fwd<64, true, kPartial>(mq, mk, mv, p, stream)
-                   : launch_fwd<64, false, kPartial>(mq, mk, mv, p, stream);
-    return f16 ? launch_fwd<128, true, kPartial>(mq, mk, mv, p, stream)
-               : launch_fwd<128, false, kPartial>(mq, mk, mv, p, stream);
+        return f16 ? launch_fwd<64, true, kPartial, kNarrow>(mq, mk, mv, p, stream)
+                   : launch_fwd<64, false, kPartial, kNarrow>(mq, mk, mv, p, stream);
+    return f16 ? launch_fwd<128, true, kPartial, kNarrow>(mq, mk, mv, p, stream)
+               : launch_fwd<128, false, kPartial, kNarrow>(mq, mk, mv, p, stream);
 }
 
 int check_window(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale) {
@@ -99,6 +99,9 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
     if ((long long)B * Hq > 0x7fffffffLL || units * p.q_blocks > 0x7fffffffLL)
         return bf_set_error(BF_ERR_ARG, "problem too large for one launch");
     p.items = (int)(units * p.q_blocks);
+    p.by_units.set((uint32_t)units);
+    p.by_heads.set((uint32_t)(p.pair_heads ? Hq / 2 : Hq));
+    p.by_group.set((uint32_t)p.group);
 
     if ((rc = bind_context()) != BF_OK) return rc;
     const bool f16 = dtype == BF_DTYPE_F16;
@@ -109,7 +112,13 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
     if ((rc = make_map_4d(&mq, Q->data, f16, dq, tq, 128, 1)) != BF_OK) return rc;
     if ((rc = make_map_4d(&mk, K->data, f16, dk, tk, 128, 1)) != BF_OK) return rc;
     if ((rc = make_map_4d(&mv, V->data, f16, dk, tv, 128, 1)) != BF_OK) return rc;
-    return launch_fwd<false>(d, f16, mq, mk, mv, p, reinterpret_cast<cudaStream_t>(stream));
+    // Sinks in a step of 32 columns where they fit one: at N = 8192 with 4 sinks, d = 64, window
+    // 1024 it takes 235 -> 209 us, d = 128, window 128 130 -> 122. At d = 128 and window 1024 it
+    // takes 303 -> 314 (the larger kernel's full steps are scheduled worse), so there only for
+    // short windows.
+    const bool narrow = p.sinks > 0 && p.sinks <= 32 && (d == 64 || p.window <= 384);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return narrow ? launch_fwd<false, true>(d, f16, mq, mk, mv, p, st) : launch_fwd<false, false>(d, f16, mq, mk, mv, p, st);
 }
 
 namespace {
@@ -319,7 +328,7 @@ int bf_prefix_partial(const PrefixArgs& a) {
         return rc;
     if ((rc = make_map_4d(&mk, a.k.data, a.f16, dk, tk, 128, 1)) != BF_OK) return rc;
     if ((rc = make_map_4d(&mv, a.v.data, a.f16, dk, tv, 128, 1)) != BF_OK) return rc;
-    return launch_fwd<true>(a.d, a.f16, mq, mk, mv, p, a.stream);
+    return launch_fwd<true, false>(a.d, a.f16, mq, mk, mv, p, a.stream);
 }
 
 int bf_window_wait_status(int reset, unsigned* out) {
