@@ -13,6 +13,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <string>
+
 #include "../../include/blackflash_b200.h"
 
 namespace {
@@ -35,7 +37,7 @@ torch::Tensor forward(const torch::Tensor& Q, const torch::Tensor& K, const torc
     const cudaStream_t stream = at::cuda::getCurrentCUDAStream(Q.device().index()).stream();
     const int rc = blackflash_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nullptr, nullptr, (int)B,
                                   (int)H, (int)N, (int)d, (float)scale, stream);
-    TORCH_CHECK(rc == BF_OK, "blackflash_fwd failed (code ", rc, "): ", blackflash_last_error());
+    TORCH_CHECK(rc == BF_OK, "blackflash_fwd failed (code ", std::to_string(rc), "): ", blackflash_last_error());
     return O;
 }
 
