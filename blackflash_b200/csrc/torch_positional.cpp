@@ -7,6 +7,7 @@
 
 #include <cmath>
 #include <limits>
+#include <string>
 
 #include "../../include/blackflash_b200.h"
 
@@ -27,15 +28,17 @@ int dtype_of(const Tensor& t) {
     }
 }
 
+// Numbers in messages go through std::to_string: streamed into a message as numbers they crash
+// the process here, inside the stream's operator<<.
 void ok(int rc, const char* what) {
-    TORCH_CHECK(rc == BF_OK, what, " failed (code ", rc, "): ", blackflash_last_error());
+    TORCH_CHECK(rc == BF_OK, what, " failed (code ", std::to_string(rc), "): ", blackflash_last_error());
 }
 
 void check(const char* name, const Tensor& t, int64_t dims, const Tensor* like = nullptr, bool fp32 = false) {
+    TORCH_CHECK(t.dim() == dims, name, " must have ", std::to_string(dims), " axes");
     const int ty = dtype_of(t);
     TORCH_CHECK(t.is_cuda() && (ty == BF_DTYPE_BF16 || ty == BF_DTYPE_F16 || (fp32 && ty == BF_DTYPE_F32)), name,
                 " must be a CUDA tensor of bfloat16", fp32 ? ", float16 or float32" : " or float16");
-    TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " axes");
     TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, "'s last axis must be contiguous");
     if (like)
         TORCH_CHECK(t.scalar_type() == like->scalar_type() && t.device() == like->device(), name,

@@ -132,6 +132,8 @@ def test_python_checks():
                  lambda: bf.prefix_decode(q, q[0], q[0], q, q, n), lambda: bf.rotary(q, q, n, f)):
         with pytest.raises(RuntimeError, match="must be a"):
             call()
+    with pytest.raises(RuntimeError, match="must have 4 axes"):  # a message with a number in it
+        bf.window_attention(q[0], q, q, 4)
     for kw in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=4, base=1.0), dict(rotary_dim=4, factor=0.5),
                dict(rotary_dim=4, scaling="cubic"), dict(rotary_dim=2, scaling="ntk", factor=2.0),
                dict(rotary_dim=4, scaling="by-parts", factor=2.0)):
