@@ -538,11 +538,20 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
         const long long tiles = per ? (B + per - 1) / per : B * ((q_rows + 127) / 128);
         const long long u = (tiles + 1) / 2 * Hkv;
         const int nk = (P + 127) / 128;
+        // The prefix blocks keep a multiprocessor each, bound by their steps; the cache's part,
+        // bound by bytes, runs on the others meanwhile and on all of them after. The split that
+        // ends first, in ns as measured: a step of two 128-row tiles, a block's start and end,
+        // the bytes a multiprocessor streams (the caches half full), a part's write and read.
+        const long long step = d == 128 ? 2200 : 1300, ends = 5000;
+        const long long cache = (long long)B * Hkv * C * d * 2 / 50;  // ns of one multiprocessor
         best = -1;
-        for (int n = 1; n <= nk && n <= 2 * kPlanSms; ++n) {
+        for (int n = 1; n <= nk && n <= 2 * kPlanSms; n += 1 + n / 16) {
             const int s = (nk + n - 1) / n, real = (nk + s - 1) / s;
-            // Waves of blocks times their steps; two steps' time to fill and drain a block.
-            const long long cost = (real * u + kPlanSms - 1) / kPlanSms * (s + 2);
+            const long long blocks = real * u, used = blocks < kPlanSms ? blocks : kPlanSms;
+            const long long t = (blocks + kPlanSms - 1) / kPlanSms * (s * step + ends);
+            const long long meanwhile = (kPlanSms - used) * t;
+            const long long after = cache > meanwhile ? (cache - meanwhile) / kPlanSms : 0;
+            const long long cost = t + after + real * p.rows * d * 8 / 3000;
             if (best < 0 || cost < best) {
                 best = cost;
                 p.p_splits = real;
