@@ -684,9 +684,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restri
                 y[k] = *reinterpret_cast<const uint4*>(d_bh + (long long)i * sn);
             }
         }
+        float mine = 0.f;  // lane k's: the sum of row k
 #pragma unroll
         for (int k = 0; k < kPrepRows; ++k) {
-            const int i = i0 + k * R;  // n_pad is a multiple of 128, and so of a pass: all rows or none
             float acc = 0.f;
             const uint32_t xs[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
 #pragma unroll
@@ -695,17 +695,19 @@ __global__ void __launch_bounds__(256) prep_kernel(const __nv_bfloat16* __restri
                        __uint_as_float(xs[c] & 0xffff0000u) * __uint_as_float(ys[c] & 0xffff0000u);
 #pragma unroll
             for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-            if (lane == 0) {
-                const float l = i < n ? lse[(size_t)bh * n + i] : -INFINITY;
-                const bool seen = l != -INFINITY;
-                const size_t r = (size_t)bh * n_pad + i;
-                nlse2[r] = seen ? -l * 1.4426950408889634f : -INFINITY;
-                nd[r] = -acc;
-                uint32_t l0, l1, l2, d0, d1, d2;
-                split3(seen ? -l * inv_scale : -1e37f, l0, l1, l2);
-                split3(-acc, d0, d1, d2);
-                aug[r] = make_uint4(l0 | (l1 << 16), l2 | (d0 << 16), d1 | (d2 << 16), 0u);
-            }
+            if (lane == k) mine = acc;
+        }
+        if (lane < kPrepRows) {
+            const int i = i0 + lane * R;  // n_pad is a multiple of 128, and so of a pass: all rows or none
+            const float l = i < n ? lse[(size_t)bh * n + i] : -INFINITY;
+            const bool seen = l != -INFINITY;
+            const size_t r = (size_t)bh * n_pad + i;
+            nlse2[r] = seen ? -l * 1.4426950408889634f : -INFINITY;
+            nd[r] = -mine;
+            uint32_t l0, l1, l2, d0, d1, d2;
+            split3(seen ? -l * inv_scale : -1e37f, l0, l1, l2);
+            split3(-mine, d0, d1, d2);
+            aug[r] = make_uint4(l0 | (l1 << 16), l2 | (d0 << 16), d1 | (d2 << 16), 0u);
         }
     }
 }
