@@ -110,9 +110,13 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     const int kvh = bh % p.hkv, b = bh / p.hkv;
     // Behind the prefix part, this grid was launched only after every grid before that one had
     // completed, and needs nothing of it. But its own completion, for which the join waits,
-    // has to mean the prefix part's too: the last block waits for it at its end.
+    // has to mean the prefix part's too: the last block waits for it at its end. The fence keeps
+    // the loads of lengths and Q from lines that L1 may still hold from before those grids.
     griddep_launch_dependents();
-    if (!p.beside) griddep_wait();
+    if (p.beside)
+        __threadfence();
+    else
+        griddep_wait();
 
     const int len = min(max(p.lengths[b], 0), p.cap);
     const int pos0 = len - p.tokens;  // position of new token 0; may be negative
@@ -127,20 +131,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     const int r0 = rt * 16 + (lane >> 2), r1 = r0 + 8;
     const int p0 = pos0 + r0 % p.tokens, p1 = pos0 + r1 % p.tokens;
     const size_t row_base = ((size_t)b * p.hkv + kvh) * p.q_rows;
-
-    // A fragments of Q: rows past the tile's last read as zero.
-    uint32_t qf[D / 16][4];
-    {
-        const uint32_t* q32 = reinterpret_cast<const uint32_t*>(p.q);
-        const size_t a0 = (row_base + r0) * (D / 2) + (lane & 3), a1 = (row_base + r1) * (D / 2) + (lane & 3);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            qf[kk][0] = r0 < p.q_rows ? q32[a0 + kk * 8] : 0u;
-            qf[kk][1] = r1 < p.q_rows ? q32[a1 + kk * 8] : 0u;
-            qf[kk][2] = r0 < p.q_rows ? q32[a0 + kk * 8 + 4] : 0u;
-            qf[kk][3] = r1 < p.q_rows ? q32[a1 + kk * 8 + 4] : 0u;
-        }
-    }
 
     uint8_t* mine = smem + warp * C::kWarpBytes;
     const uint32_t mine_a = smem_addr(mine);
@@ -180,6 +170,21 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
 
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) load(s);
+
+    // A fragments of Q, requested behind the first keys: rows past the tile's last read as zero.
+    uint32_t qf[D / 16][4];
+    {
+        const uint32_t* q32 = reinterpret_cast<const uint32_t*>(p.q);
+        const size_t a0 = (row_base + r0) * (D / 2) + (lane & 3), a1 = (row_base + r1) * (D / 2) + (lane & 3);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][0] = r0 < p.q_rows ? q32[a0 + kk * 8] : 0u;
+            qf[kk][1] = r1 < p.q_rows ? q32[a1 + kk * 8] : 0u;
+            qf[kk][2] = r0 < p.q_rows ? q32[a0 + kk * 8 + 4] : 0u;
+            qf[kk][3] = r1 < p.q_rows ? q32[a1 + kk * 8 + 4] : 0u;
+        }
+    }
+
     for (int s = 0; s < steps; ++s) {
         load(s + kStages - 1);
         cp_async_wait<kStages - 1>();

@@ -145,12 +145,16 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     const long long total = units * ((p.nk - p.ns) * norm + p.ns * sink);
     // Two items a multiprocessor where the work allows it, none shorter than 16 steps (below
     // that a part's own fp32 output weighs more than what it reads). The blocks take items in
-    // turn, so a sink tile comes in parts of about the other items' length.
+    // turn, so a sink tile comes in parts of about the other items' length, in all at most
+    // eight parts a multiprocessor beside whole tiles (that bounds the workspace: 1184 parts are
+    // 155 MB at d = 128).
     long long target = (total + 2 * kPlanSms - 1) / (2 * kPlanSms);
     if (target < 16) target = 16;
     p.splits_n = norm * 2 > target * 3 ? (int)((norm + target - 1) / target) : 1;
     const long long floor_s = target < 64 ? target : 64;
-    const long long target_s = p.splits_n > 1 ? target : (norm > floor_s ? norm : floor_s);
+    long long target_s = p.splits_n > 1 ? target : (norm > floor_s ? norm : floor_s);
+    const long long least = (units * p.ns * sink + 8 * kPlanSms - 1) / (8 * kPlanSms);
+    if (target_s < least) target_s = least;
     p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
     // D from fp32 sums where a row sees at most a tile of keys: there the rounding of O would
     // dominate the error of dQ and dK.

@@ -149,6 +149,37 @@ def test_refusals_on_the_gpu():
     assert torch.isfinite(bf.window_attention(q, k, k, 4)).all()
 
 
+FIRST_CALLS = """
+import torch
+import blackflash_b200 as bf
+q = torch.randn(2, 4, 200, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+k, n = q.detach()[:, :2], torch.tensor([200, 77], dtype=torch.int32, device="cuda")
+freqs, _ = bf.rotary_frequencies(64)
+pos = torch.arange(200, device="cuda")
+def calls():
+    o = bf.window_attention_with_grad(q, k, k, 50, 4)
+    return [o.detach(), torch.autograd.grad(o, q, torch.ones_like(o))[0], *bf.rotary(q.detach(), k, pos, freqs),
+            bf.window_decode(q.detach()[:, :, :1], k, k, n, 50, 4), bf.prefix_decode(q.detach()[:, :, :1], k[0], k[0], k, k, n)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """Set-up that a first call does (kernel attributes, entry points) is allowed in a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_other_device_than_the_current():
     import blackflash_b200 as bf

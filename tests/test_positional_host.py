@@ -31,6 +31,10 @@ def test_window_backward_plans(lib, change):
     many = ws(*{**ok, "Nq": 12800, "Nkv": 12800, "sinks": 4}.values()) - 4 * 6 * 4 * 12800
     assert many > 0 and many % (2 * 128 * 64 * 4) == 0
     assert ws(*{**ok, **change}.values()) == -1 and lib.blackflash_last_error()
+    # Long, and with a whole length of sinks: the parts stay bounded, whatever the length.
+    for n, sinks in ((1 << 20, 4), (1 << 20, 128), (1 << 16, 1 << 16), (1 << 20, 1 << 20)):
+        parts = ws(1, 8, 8, n, n, 128, 64, sinks) - 4 * 6 * 8 * n
+        assert 0 <= parts <= (8 * 148 + 8 * 148) * 2 * 128 * 128 * 4
 
 
 def test_window_backward_refusals(lib):
