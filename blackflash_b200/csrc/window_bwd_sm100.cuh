@@ -19,9 +19,10 @@
 //   dQ    (kDQ=1)    Q   dO   K   V                                  dQ += dS Y0
 // D. Both passes read it from an array that the prep kernel fills from O. O is rounded to
 // bf16, and for a row that sees few keys that error is not small against dP - D, of which D
-// is then a large part (one key: dP - D is 0). So with few keys (two_sweeps) the dQ pass
-// walks its KV tiles twice: first it sums P dP and P in fp32, D = sum P dP / sum P, which it
-// also leaves in the array for the dK/dV pass; then it accumulates.
+// is then a large part (one key: dP - D is 0). So a query tile with such a row (the first of a
+// sequence, or every one of a short window) walks its KV tiles twice in the dQ pass: first it
+// sums P dP and P in fp32, D = sum P dP / sum P, which it also leaves in the array for the
+// dK/dV pass; then it accumulates.
 // Roles: two groups of eight elementwise warps (two threads per row), which take the steps in
 // turn: a step is a chain of TMEM loads, exponentials and stores that one group alone leaves
 // mostly waiting, so the other one's chain runs under it; a TMA producer; one issuer each of S,
@@ -53,6 +54,7 @@ constexpr int kEwRegs = 104, kOtherRegs = 64;  // launch budget 640 x 96
 static_assert(kEwWarps * 32 * kEwRegs + 128 * kOtherRegs <= kThreads * 96, "register split exceeds the launch budget");
 constexpr int NT = 64;       // rows of a streamed tile
 constexpr int NC = NT / 2;   // of them (S columns) a thread's
+constexpr int kFewKeys = 128;  // D from fp32 sums for tiles with a row that sees at most so many
 constexpr int kBufs = 4;     // S / dP / P, dS buffers; step n uses buffer n % 4
 constexpr int kColAcc = kBufs * NT;
 
@@ -124,7 +126,6 @@ struct Params {
     const float* nlse2;      // [B Hq, n_pad] -lse log2(e); -inf past n_q and for rows that see nothing
     const float* nd;         // [B Hq, n_pad] -D
     uint4* aug;              // [B Hq, n_pad] eight bf16: -lse / scale in three terms, -D in three, 0, 0
-    int two_sweeps;          // dQ: find D in a first sweep over the KV tiles, and store it in aug
     __nv_bfloat16 *dq, *dk, *dv;
     float* part;             // [slot][dV, dK][128][D] of the tiles with more than one part
     unsigned long long timeout_ns;
@@ -134,6 +135,7 @@ struct Item {
     int b, kvh, head;   // head: the query head (dQ)
     int tile;           // stationary 128-row tile
     int steps;          // dQ: of one sweep
+    int lead;           // dQ: steps of a first sweep, which finds D and stores it in aug, or 0
     int i0, ni, s0;     // dK/dV: step s is query tile i0 + (s0 + s) % ni of head (s0 + s) / ni
     int n_sink, skip;   // dQ: step s is KV tile s, or s + skip past the sink tiles
     long long slot;     // dK/dV: part to write, -1: the gradient itself
@@ -175,8 +177,11 @@ __device__ __forceinline__ void decode(const Params& p, int item, Item& it) {
         it.n_sink = min((p.sinks + NT - 1) / NT, lo);
         it.skip = lo - it.n_sink;
         it.steps = hi > 0 ? hi - it.skip : 0;
+        // The tile's first row sees min(p_first + 1, window + sinks) keys, the fewest of its rows.
+        it.lead = p_first < kFewKeys || p.window <= kFewKeys - p.sinks ? it.steps : 0;
         it.slot = -1;
     } else {
+        it.lead = 0;
         // Sink tiles first, in parts (all later queries see them); early keys are seen most.
         const int units = p.batch * p.hkv;
         const int unit = item % units;
@@ -284,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t sl2_2 = f2_pack(p.scale_log2, p.scale_log2);
         uint32_t n0 = 0;  // steps of the items before
         int n_it = 0;     // items with steps so far
+        int n_swept = 0;  // of them with a first sweep
         bool ok = true;
         // dQ: the next item is decoded, and its rows' -lse2 and -D requested, before the current
         // one's gradients are waited for (dK/dV has more steps an item and no registers for it).
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (kDQ) {
                 const size_t at = ((size_t)next.b * p.hq + next.head) * p.n_pad + next.tile * 128 + row;
                 next_l = p.nlse2[at];
-                next_d = p.two_sweeps ? 0.f : p.nd[at];
+                next_d = next.lead > 0 ? 0.f : p.nd[at];
             }
         };
         if constexpr (kDQ) fetch(blockIdx.x);
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (!kDQ) fetch(item);
             const Item it = next;
             const int xrow = it.tile * 128 + row;
-            const int lead = kDQ && p.two_sweeps ? it.steps : 0;  // steps of the first sweep
+            const int lead = it.lead;
             uint64_t nl2 = f2_pack(next_l, next_l), nd2 = f2_pack(next_d, next_d);
             int q_tile = 0;  // dK/dV: the next step's query tile, from i0 on
             // One step; in the first sweep (measure) it only adds up P and P dP.
@@ -393,11 +399,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // D from the four sums of the row: two column halves, two groups.
                     sum_p += __shfl_xor_sync(0xffffffffu, sum_p, 16);
                     sum_pdp += __shfl_xor_sync(0xffffffffu, sum_pdp, 16);
-                    float2* sums = reinterpret_cast<float2*>(smem + C::kOffSum) + (n_it & 1) * 256;
+                    float2* sums = reinterpret_cast<float2*>(smem + C::kOffSum) + (n_swept & 1) * 256;
                     if (h == 0) sums[grp * 128 + row] = make_float2(sum_p, sum_pdp);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_addr(&bars->sums));
-                    if (!(ok = warp_wait(smem_addr(&bars->sums), (uint32_t)n_it & 1u, ctl, kSiteEwSums))) break;
+                    if (!(ok = warp_wait(smem_addr(&bars->sums), (uint32_t)n_swept & 1u, ctl, kSiteEwSums))) break;
+                    ++n_swept;
                     const float2 x = sums[row], y = sums[128 + row];
                     const float tp = x.x + y.x, tpdp = x.y + y.y;
                     const float b = tp != 0.f ? -tpdp / tp : 0.f;  // a row that sees nothing has D = 0
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ++n_it;
             __syncwarp();
-            const int lead = kDQ && p.two_sweeps ? it.steps : 0;
+            const int lead = it.lead;
             int g = 0, i = 0;  // dK/dV: head of the group and query tile of the next step
             if constexpr (!kDQ) {
                 g = it.s0 / it.ni;
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Item it;
             decode<D, kDQ>(p, item, it);
             if (it.steps == 0) continue;
-            const int lead = kDQ && p.two_sweeps ? it.steps : 0, last = lead + it.steps - 1;
+            const int lead = it.lead, last = lead + it.steps - 1;
             if (role < 2) {
                 if (!(ok = warp_wait(smem_addr(&bars->x_full), (uint32_t)n_it & 1u, ctl, kSiteFrontX))) break;
                 tc_fence_after();

@@ -127,7 +127,6 @@ namespace {
 struct BwdPlan {
     int nk, ns, window, sinks, n_pad, splits_s, splits_n;
     long long vec, slots, bytes;
-    bool two_sweeps;
 };
 
 BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks) {
@@ -156,9 +155,6 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     const long long least = (units * p.ns * sink + 8 * kPlanSms - 1) / (8 * kPlanSms);
     if (target_s < least) target_s = least;
     p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
-    // D from fp32 sums where a row sees at most a tile of keys: there the rounding of O would
-    // dominate the error of dQ and dK.
-    p.two_sweeps = p.window + p.sinks <= 128;
     p.vec = (long long)B * Hq * p.n_pad;
     p.slots = units * ((p.splits_s > 1 ? (long long)p.ns * p.splits_s : 0) +
                        (p.splits_n > 1 ? (long long)(p.nk - p.ns) * p.splits_n : 0));
@@ -227,10 +223,11 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
         const int per = 256 / (d / 8) * bfk::winb::kPrepRows;  // rows of a block: divides 128
         const int chunks = plan.n_pad / per;
         const dim3 grid((unsigned)(B * Hq), (unsigned)(chunks < 65535 ? chunks : 65535));
+        const bool all_swept = plan.window <= bfk::winb::kFewKeys - plan.sinks;  // D comes from the dQ pass
         auto kernel = d == 64 ? bfk::winb::prep_kernel<64> : bfk::winb::prep_kernel<128>;
         if ((rc = launch_error(launch_pdl(kernel, grid, 256, 0, st, reinterpret_cast<const __nv_bfloat16*>(O),
                                           reinterpret_cast<const char*>(dO->data), sd.s[0] * 2, sd.s[1] * 2, sd.s[2] * 2, lse,
-                                          nlse2, nd, aug, 1.f / scale, Hq, Nq, plan.n_pad, plan.two_sweeps ? 0 : 1))) != BF_OK)
+                                          nlse2, nd, aug, 1.f / scale, Hq, Nq, plan.n_pad, all_swept ? 0 : 1))) != BF_OK)
             return rc;
     }
     const long long dq[4] = {d, Nq, Hq, B}, dk[4] = {d, Nkv, Hkv, B};
@@ -262,7 +259,6 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.q_tiles = q_tiles;
     p.splits_s = plan.splits_s;
     p.splits_n = plan.splits_n;
-    p.two_sweeps = plan.two_sweeps;
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
     p.nlse2 = nlse2;
@@ -273,7 +269,7 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.dv = reinterpret_cast<__nv_bfloat16*>(dV);
     p.part = part;
     p.timeout_ns = kTimeoutNs;
-    p.items = (int)q_items;  // first: it may leave a better D
+    p.items = (int)q_items;  // first: it leaves a better D of rows that see few keys
     rc = d == 64 ? launch_bwd<64, true>(mq[0], md[0], mk[1], mv[1], p, st)
                  : launch_bwd<128, true>(mq[0], md[0], mk[1], mv[1], p, st);
     if (rc != BF_OK) return rc;

@@ -257,3 +257,19 @@ def test_window_backward_empty():
     q, k = z(2, 4, 3, 64), z(2, 2, 0, 64)
     dq, dk, dv = window_attention_backward(q, k, k, q, q, torch.zeros(2, 4, 3, device="cuda"), 5)
     assert (dq == 0).all() and dk.shape == dv.shape == k.shape
+
+
+@pytest.mark.parametrize("d,n,window,sinks", [(64, 300, 200, 4), (128, 618, 568, 0), (64, 700, 64, 65)])
+def test_one_key_has_no_score_gradient(d, n, window, sinks):
+    """The first row sees one key: P = 1, so dP - D is 0 whatever O was rounded to. In fp32,
+    D = (P dP) / P is dP to three roundings of 2^-24 (two products, one quotient; P is 1 to a
+    few 2^-22 and cancels), and dS = P (dP - D) rounds once more: 2^-21 |dP| holds them."""
+    import blackflash_b200 as bf
+    q, k, v = make(2, 6, 2, n, n, d)
+    do = make(2, 6, 2, n, n, d, seed=1)[0]
+    o, lse = bf.window_attention_lse(q, k, v, window, sinks)
+    dq, _, _ = bf.window_attention_backward(q, k, v, o, do, lse, window, sinks)
+    k0, v0 = (x[:, :, :1].double().repeat_interleave(3, 1) for x in (k, v))
+    dp = (do[:, :, :1].double() * v0).abs().sum(-1, keepdim=True)  # at least |dP|, in either sweep's sum
+    bound = d ** -0.5 * dp * k0.abs() * 2.0 ** -21
+    assert (dq[:, :, :1].double().abs() <= bound).all()
