@@ -2,6 +2,7 @@
 // outputs, workspaces and autograd nodes in C++ over the C ABI, because a decoding step or a
 // short training step takes the GPU less time than the same work takes the interpreter.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -138,9 +139,20 @@ Tensor rows(const Tensor& t) {
     return fine ? t : t.contiguous();
 }
 
-void once() {
+// What a backward refuses. A node keeps the stream that it was made on, a leaf's too while any
+// graph of the leaf lives; the engine would have the default stream wait for a captured one,
+// which ends the capture and, on the engine's thread, the process.
+void check_backward() {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "this operator is differentiable once: its backward does not support create_graph=True");
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    for (const auto& edge : node->next_edges()) {
+        const auto stream = edge.function ? edge.function->stream() : c10::nullopt;
+        TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                    "a backward cannot be captured while a graph of its inputs from the default stream is alive: drop that "
+                    "graph first, or make it on another stream");
+    }
 }
 
 struct WindowFn : torch::autograd::Function<WindowFn> {
@@ -154,7 +166,7 @@ struct WindowFn : torch::autograd::Function<WindowFn> {
         return o;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once();
+        check_backward();
         const variable_list s = ctx->get_saved_variables();
         auto [dq, dk, dv] = window_backward(s[0], s[1], s[2], s[3], rows(grads[0]), s[4], ctx->saved_data["window"].toInt(),
                                             ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toOptional<double>());
@@ -276,7 +288,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
         return {qo, ko};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once();
+        check_backward();
         // The map is linear, so its gradient is its transpose: the same turn backwards.
         const variable_list s = ctx->get_saved_variables();
         auto [dq, dk] = rotary(pairs(grads[0]), pairs(grads[1]), s[0], s[1], ctx->saved_data["interleaved"].toBool(),

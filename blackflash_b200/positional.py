@@ -75,7 +75,10 @@ def window_attention_backward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
 
 def window_attention_with_grad(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, window: int, sinks: int = 0,
                                scale: float | None = None) -> torch.Tensor:
-    """`window_attention` as a differentiable op (once: no create_graph); bf16."""
+    """`window_attention` as a differentiable op (once: no create_graph); bf16.
+
+    Forward and backward may be captured together into a CUDA graph, except while a graph of
+    the same leaves that was made on the default stream is alive: that backward is refused."""
     _tensors(Q=Q, K=K, V=V)
     return _ext().window_with_grad(Q, K, V, min(window, _MAX), min(sinks, _MAX), scale)
 
@@ -173,6 +176,6 @@ def rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, freqs: tor
 def rotary_with_grad(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
                      interleaved: bool = False, amplitude: float = 1.0):
     """`rotary` as a differentiable op (once: no create_graph); gradients for Q and K, not for
-    the frequencies."""
+    the frequencies. For CUDA graphs as `window_attention_with_grad`."""
     _tensors(Q=Q, K=K, positions=positions, freqs=freqs)
     return _ext().rotary_with_grad(Q, K, positions, freqs, interleaved, amplitude)

@@ -180,6 +180,55 @@ def test_first_calls_of_a_process_under_capture():
     assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
 
 
+CAPTURED_LEAF = """
+import torch
+import blackflash_b200 as bf
+q = torch.randn(2, 4, 200, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+k = torch.randn(2, 2, 200, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+freqs, _ = bf.rotary_frequencies(64)
+pos = torch.arange(200, device="cuda")
+forms = {"window": lambda: bf.window_attention_with_grad(q, k, k, 50, 4),
+         "rotary": lambda: bf.rotary_with_grad(q, k, pos, freqs)[0]}
+grad = torch.ones_like(q)
+def step(form):
+    return torch.autograd.grad(form(), [q, k], grad)
+for name, form in forms.items():
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(form)
+    torch.cuda.current_stream().wait_stream(side)
+    alive = form()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            step(form)
+    except RuntimeError as e:
+        assert "graph of its inputs" in str(e), e
+        print("refused", name, flush=True)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(form)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, step(form)))
+    print("captured", name, flush=True)
+"""
+
+
+def test_captured_backward_beside_an_eager_graph_of_its_leaves():
+    """Refused, in words, and captured once that graph is gone; in a process of its own, which
+    the engine's failure would end."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", CAPTURED_LEAF], cwd=root, capture_output=True, text=True, timeout=300)
+    lines = [f"{what} {name}" for name in ("window", "rotary") for what in ("refused", "captured")]
+    assert out.returncode == 0 and out.stdout.split("\n")[:-1] == lines, out.stdout + out.stderr[-2000:]
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_other_device_than_the_current():
     import blackflash_b200 as bf
