@@ -116,6 +116,9 @@ enum : unsigned {
 
 struct Params {
     int items;
+    // dK/dV: blocks take their items at places blockIdx, blockIdx + gridDim, .. of a list that has
+    // `late_rows` rows, from place late_from on, with holes for its first late_blocks blocks.
+    int places, late_from, late_rows, late_blocks;
     int batch, hq, hkv, group;
     int n_q, n_kv, n_pad;    // n_pad: n_q rounded up to 128, row stride of nlse2 / nd
     int nk, ns;              // KV tiles; of them tiles that hold sinks
@@ -158,6 +161,16 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
     mid = pack_bf16x2(x, 0.f) & 0xffffu;
     x -= __uint_as_float(mid << 16);
     lo = pack_bf16x2(x, 0.f) & 0xffffu;
+}
+
+// The item at a place of the list; at a hole or past the last item p.items.
+template <bool kDQ>
+__device__ __forceinline__ int item_at(const Params& p, int place) {
+    if (kDQ || place < p.late_from) return place;
+    const int row = (place - p.late_from) / (int)gridDim.x, gap = p.late_blocks;
+    if (row >= p.late_rows) return min(place - p.late_rows * gap, p.items);
+    const int item = place - (row + 1) * gap;  // of the blocks from `gap` on
+    return (int)blockIdx.x < gap ? p.items : min(item, p.items);
 }
 
 template <int D, bool kDQ>
@@ -305,7 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         };
         if constexpr (kDQ) fetch(blockIdx.x);
-        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        for (int place = blockIdx.x; place < p.places && ok; place += gridDim.x) {
+            const int item = item_at<kDQ>(p, place);
+            if (item >= p.items) continue;
             if constexpr (!kDQ) fetch(item);
             const Item it = next;
             const int xrow = it.tile * 128 + row;
@@ -488,7 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         int n_it = 0, n = 0, st = 0;
         uint32_t par = 1u;
         bool ok = true;
-        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        for (int place = blockIdx.x; place < p.places && ok; place += gridDim.x) {
+            const int item = item_at<kDQ>(p, place);
+            if (item >= p.items) continue;
             Item it;
             decode<D, kDQ>(p, item, it);
             if (it.steps == 0) continue;
@@ -575,7 +592,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t n = 0, st = 0, par = 0;     // step, its stage and the stage's parity
         int n_it = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        for (int place = blockIdx.x; place < p.places && ok; place += gridDim.x) {
+            const int item = item_at<kDQ>(p, place);
+            if (item >= p.items) continue;
             Item it;
             decode<D, kDQ>(p, item, it);
             if (it.steps == 0) continue;

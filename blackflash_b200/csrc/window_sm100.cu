@@ -126,6 +126,7 @@ namespace {
 // How the dK/dV pass is split, and its workspace: -lse2 and -D, both as terms, then the parts.
 struct BwdPlan {
     int nk, ns, window, sinks, n_pad, splits_s, splits_n;
+    int times;  // a sink tile's part has the length of so many parts of other tiles
     long long vec, slots, bytes;
 };
 
@@ -143,10 +144,11 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     const long long norm = group * ((seen + nt - 1) / nt), sink = group * ((Nq + nt - 1) / nt);
     const long long total = units * ((p.nk - p.ns) * norm + p.ns * sink);
     // Two items a multiprocessor where the work allows it, none shorter than 16 steps (below
-    // that a part's own fp32 output weighs more than what it reads). The blocks take items in
-    // turn, so a sink tile comes in parts of about the other items' length, in all at most
-    // eight parts a multiprocessor beside whole tiles (that bounds the workspace: 1184 parts are
-    // 155 MB at d = 128).
+    // that a part's own fp32 output weighs more than what it reads). A sink tile stays whole
+    // where it is no longer than a multiprocessor's mean (in parts of 64 steps: 1 to 8 % slower,
+    // the join's time and launch). A longer one comes in parts of about the other items'
+    // length, in all at most eight parts a multiprocessor beside whole tiles (that bounds the
+    // workspace: 1184 parts are 155 MB at d = 128).
     long long target = (total + 2 * kPlanSms - 1) / (2 * kPlanSms);
     if (target < 16) target = 16;
     p.splits_n = norm * 2 > target * 3 ? (int)((norm + target - 1) / target) : 1;
@@ -154,7 +156,10 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     long long target_s = p.splits_n > 1 ? target : (norm > floor_s ? norm : floor_s);
     const long long least = (units * p.ns * sink + 8 * kPlanSms - 1) / (8 * kPlanSms);
     if (target_s < least) target_s = least;
+    if (p.splits_n == 1 && sink * kPlanSms <= total) target_s = sink;
     p.splits_s = sink * 2 > target_s * 3 ? (int)((sink + target_s - 1) / target_s) : 1;
+    const long long len_s = sink / p.splits_s, len_n = norm / p.splits_n;
+    p.times = (int)((len_s + len_n / 2) / (len_n > 0 ? len_n : 1));
     p.vec = (long long)B * Hq * p.n_pad;
     p.slots = units * ((p.splits_s > 1 ? (long long)p.ns * p.splits_s : 0) +
                        (p.splits_n > 1 ? (long long)(p.nk - p.ns) * p.splits_n : 0));
@@ -162,15 +167,39 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     return p;
 }
 
+// `first`: dK/dV items of sink tiles, which come first, and how many times the others' length they
+// have. Blocks that begin with one of them take so many items less of the others: with all in
+// turn, 32 blocks at B=2 H=16 N=4096 window 1024 had 172 steps where the mean is 134 (the
+// backward there, d = 64: 240 -> 224 us; d = 128 window 512: 226 -> 203).
+struct FirstItems {
+    long long count;
+    int times;
+};
+
 template <int D, bool kDQ>
 int launch_bwd(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0, const CUtensorMap& y1,
-               const bfk::winb::Params& p, cudaStream_t stream) {
+               bfk::winb::Params p, FirstItems first, cudaStream_t stream) {
     static std::atomic<bool> done[64];  // per device; zero-initialised (static storage)
     auto kernel = bfk::winb::window_bwd_kernel<D, kDQ>;
     int rc, sms = 0;
     if ((rc = allow_smem(kernel, bfk::winb::smem_bytes<D, kDQ>(), done)) != BF_OK) return rc;
     if ((rc = sm_count(&sms)) != BF_OK) return rc;
     const int grid = p.items < sms ? p.items : sms;  // persistent: one block per multiprocessor
+    p.places = p.late_from = p.items;
+    const int late = (int)(first.count % grid);
+    if (late > 0 && first.times > 1) {
+        // The row of the list in which `late` blocks still have a first item gives the others one
+        // item; after it come times - 1 rows for them alone, while there are items.
+        const long long from = first.count - late + grid, rest = p.items - from;
+        const long long rows = rest > 0 ? (rest + grid - late - 1) / (grid - late) : 0;
+        const long long late_rows = rows < first.times - 1 ? rows : first.times - 1;
+        if (p.items + late_rows * late <= 0x7fffffffLL - grid) {
+            p.late_from = (int)(from < p.items ? from : p.items);
+            p.late_rows = (int)late_rows;
+            p.late_blocks = late;
+            p.places = (int)(p.items + late_rows * late);
+        }
+    }
     return launch_error(launch_pdl(kernel, dim3((unsigned)grid), bfk::winb::kThreads, bfk::winb::smem_bytes<D, kDQ>(),
                                    stream, x0, x1, y0, y1, p));
 }
@@ -270,12 +299,13 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     p.part = part;
     p.timeout_ns = kTimeoutNs;
     p.items = (int)q_items;  // first: it leaves a better D of rows that see few keys
-    rc = d == 64 ? launch_bwd<64, true>(mq[0], md[0], mk[1], mv[1], p, st)
-                 : launch_bwd<128, true>(mq[0], md[0], mk[1], mv[1], p, st);
+    rc = d == 64 ? launch_bwd<64, true>(mq[0], md[0], mk[1], mv[1], p, {0, 0}, st)
+                 : launch_bwd<128, true>(mq[0], md[0], mk[1], mv[1], p, {0, 0}, st);
     if (rc != BF_OK) return rc;
     p.items = (int)kv_items;
-    rc = d == 64 ? launch_bwd<64, false>(mk[0], mv[0], mq[1], md[1], p, st)
-                 : launch_bwd<128, false>(mk[0], mv[0], mq[1], md[1], p, st);
+    const FirstItems first{units * plan.ns * plan.splits_s, plan.times};
+    rc = d == 64 ? launch_bwd<64, false>(mk[0], mv[0], mq[1], md[1], p, first, st)
+                 : launch_bwd<128, false>(mk[0], mv[0], mq[1], md[1], p, first, st);
     if (rc != BF_OK) return rc;
     auto join = [&](const float* from, int j0, int tiles, int splits) -> int {
         if (splits <= 1 || tiles <= 0) return BF_OK;

@@ -273,3 +273,19 @@ def test_one_key_has_no_score_gradient(d, n, window, sinks):
     dp = (do[:, :, :1].double() * v0).abs().sum(-1, keepdim=True)  # at least |dP|, in either sweep's sum
     bound = d ** -0.5 * dp * k0.abs() * 2.0 ** -21
     assert (dq[:, :, :1].double().abs() <= bound).all()
+
+
+@pytest.mark.parametrize("b,h,n,window,sinks", [
+    (2, 20, 1500, 100, 3),    # fewer sink tiles than blocks, each as long as six others
+    (1, 150, 700, 65, 1),     # two blocks have a second sink tile
+    (3, 50, 513, 129, 130),   # two sink tiles a head
+    (1, 80, 257, 30, 257),    # nothing but sink tiles
+    (1, 140, 300, 30, 2),     # blocks without a sink tile are few
+])
+def test_window_backward_late_blocks(b, h, n, window, sinks):
+    """Items of unlike length dealt to the blocks: every tile has its gradient, each time the same."""
+    q, k, v = make(b, h, h, n, n, 64)
+    do = upstream(q)
+    got = grads_of(q, k, v, do, window, sinks)
+    check_grads(got, q, k, v, do, window, sinks)
+    assert all(torch.equal(x, y) for x, y in zip(got, grads_of(q, k, v, do, window, sinks)))
