@@ -52,6 +52,9 @@ struct Params {
     int hkv, q_rows, tokens, cap, row_tiles;
     int window, sinks;  // clamped to cap
     int chunk;          // keys of a split
+    const char *kp, *vp;          // kPrefix: the shared prefix, whose keys come before the cache's
+    long long kps[2], vps[2];     // byte strides of head, token
+    int prefix;
     int beside;         // the grid before is the prefix part: do not wait for it at the start
     float scale_log2;
 };
@@ -98,7 +101,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return kF16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
 
-template <int D, bool kF16>
+// kPrefix: the prefix's keys are the first of the numbering, as sinks are, and every token sees
+// them; each sequence reads them for itself.
+template <int D, bool kF16, bool kPrefix>
 __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     using C = Cfg<D>;
     constexpr int NB = C::kKeys / 8;  // score blocks of 8 keys
@@ -118,10 +123,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     else
         griddep_wait();
 
-    const int len = min(max(p.lengths[b], 0), p.cap);
+    const int len = kPrefix && p.cap == 0 ? 0 : min(max(p.lengths[b], 0), p.cap);
     const int pos0 = len - p.tokens;  // position of new token 0; may be negative
     const int lo = max(0, pos0 - p.window + 1);
-    const int s0 = min(p.sinks, lo);
+    const int s0 = kPrefix ? p.prefix : min(p.sinks, lo);
     const int n_vis = s0 + len - lo;
     const long long base = (long long)split * p.chunk;
     const int v0 = base < n_vis ? (int)base : n_vis;
@@ -136,6 +141,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     const uint32_t mine_a = smem_addr(mine);
     const char* kb = p.k + b * p.ks[0] + kvh * p.ks[1];
     const char* vb = p.v + b * p.vs[0] + kvh * p.vs[1];
+    const char* kpb = kPrefix ? p.kp + kvh * p.kps[0] : nullptr;
+    const char* vpb = kPrefix ? p.vp + kvh * p.vps[0] : nullptr;
     const int groups = (v1 - v0 + C::kKeys - 1) / C::kKeys;
     const int steps = groups > warp ? (groups - warp + kWarps - 1) / kWarps : 0;
 
@@ -150,9 +157,17 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
                 const bool valid = vg + row < v1;
                 const int v = valid ? vg + row : v0;  // a safe address; nothing is read from it
                 const long long key = v < s0 ? v : lo + (v - s0);
+                const char *k_row, *v_row;
+                if (kPrefix && v < s0) {
+                    k_row = kpb + key * p.kps[1];
+                    v_row = vpb + key * p.vps[1];
+                } else {
+                    k_row = kb + key * p.ks[2];
+                    v_row = vb + key * p.vs[2];
+                }
                 const uint32_t at = (uint32_t)row * C::kRow + (uint32_t)((ch ^ (row & 7)) << 4);
-                cp_async16(dst + at, kb + key * p.ks[2] + ch * 16, valid);
-                cp_async16(dst + C::kHalf + at, vb + key * p.vs[2] + ch * 16, valid);
+                cp_async16(dst + at, k_row + ch * 16, valid);
+                cp_async16(dst + C::kHalf + at, v_row + ch * 16, valid);
             }
         }
         cp_async_commit();
@@ -223,9 +238,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
                     const int v = vg + i * 8 + (lane & 3) * 2 + e;
                     const int key = v < s0 ? v : lo + (v - s0);
                     const bool in = v < v1;
-                    const bool sink = key < p.sinks;
-                    if (!(in && key <= p0 && (sink || p0 - key < p.window))) a = -INFINITY;
-                    if (!(in && key <= p1 && (sink || p1 - key < p.window))) c = -INFINITY;
+                    const bool sink = kPrefix ? v < s0 : key < p.sinks;
+                    const bool before0 = (kPrefix && sink) || key <= p0, before1 = (kPrefix && sink) || key <= p1;
+                    if (!(in && before0 && (sink || p0 - key < p.window))) a = -INFINITY;
+                    if (!(in && before1 && (sink || p1 - key < p.window))) c = -INFINITY;
                 }
                 sc[i][e] = a;
                 sc[i][e + 2] = c;
@@ -483,6 +499,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const CombineP
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Up to so many bytes, counted anew for each sequence, a prefix is read with the sequences' own
+// keys (from L2, after the first) by one kernel: us in a graph so / with the prefix's own kernel,
+//   2.3 MB (B=4 Hq=8 Hkv=2 P=1000 d=64) 5.6 / 7.9     17 MB (B=1 Hq=8 Hkv=8 P=4096 d=128) 8.2 / 13.5
+//   30 MB (B=16 Hq=32 Hkv=8 P=200 d=128) 10.5 / 10.3  41 MB (B=8 Hq=32 Hkv=8 P=1000 d=128) 12.2 / 10.8
+// and one launch less, which is 3 us of the host's.
+constexpr long long kTogetherBytes = 32LL << 20;
 
 // How a step is split. A function of its sizes alone, so that the workspace can be sized
 // ahead of the call.
@@ -491,7 +513,8 @@ struct Plan {
     int row_tiles;        // 16-row tiles of a KV head
     int chunk, splits;    // cache: keys of a split, splits
     int p_splits, p_tiles;  // prefix: splits, KV tiles of a split
-    bool direct;          // one split, no prefix: the kernel writes O itself
+    bool together;        // the prefix's keys are read with each sequence's own, by one kernel
+    bool direct;          // one split, no prefix part: the kernel writes O itself
     long long bytes;
 };
 
@@ -512,6 +535,10 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
     // The longest run of keys a row tile can see.
     long long vis = (long long)window + T - 1 + sinks;
     if (vis > C) vis = C;
+    // A short prefix is not worth a kernel of its own, which reads it once for the batch but
+    // takes a launch, its start and parts to join.
+    p.together = P > 0 && units * (P + vis) * d * 4 <= kTogetherBytes;
+    if (p.together) vis += P;
     // Splits: blocks run three a multiprocessor, a unit's splits one grid row after the other, so
     // that the last, shorter ones fill up what the others leave. The time of a chunk size, in
     // keys of streaming: the work over the slots and a last block, at least one block; `start`
@@ -538,7 +565,7 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
         }
     }
     p.p_splits = p.p_tiles = 0;
-    if (P > 0) {
+    if (P > 0 && !p.together) {
         const long long per = 128 / q_rows;
         const long long tiles = per ? (B + per - 1) / per : B * ((q_rows + 127) / 128);
         const long long u = (tiles + 1) / 2 * Hkv;
@@ -569,11 +596,11 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
     return BF_OK;
 }
 
-template <int D, bool kF16>
+template <int D, bool kF16, bool kPrefix>
 int launch_decode(const bfk::dec::Params& p, int splits, long long units, cudaStream_t stream) {
     static std::atomic<bool> done[64];  // per device; zero-initialised (static storage)
     int rc;
-    auto kernel = bfk::dec::decode_kernel<D, kF16>;
+    auto kernel = bfk::dec::decode_kernel<D, kF16, kPrefix>;
     if ((rc = allow_smem(kernel, bfk::dec::Cfg<D>::kSmem, done)) != BF_OK) return rc;
     return launch_error(launch_pdl(kernel, dim3((unsigned)units, (unsigned)splits), bfk::dec::kWarps * 32,
                                    bfk::dec::Cfg<D>::kSmem, stream, p));
@@ -612,8 +639,12 @@ int decode_step(const StepArgs& a) {
         if ((rc = check_view(a.k, "K_cache", a.B, a.Hkv, a.C, a.d, 2, &sk)) != BF_OK) return rc;
         if ((rc = check_view(a.v, "V_cache", a.B, a.Hkv, a.C, a.d, 2, &sv)) != BF_OK) return rc;
     }
+    ViewStrides skp, svp;
     if (a.P > 0) {
-        if (!a.kp || !a.vp) return bf_set_error(BF_ERR_ARG, "prefix: null pointer");
+        if ((rc = check_view(a.kp, "K_prefix", 1, a.Hkv, a.P, a.d, 2, &skp)) != BF_OK) return rc;
+        if ((rc = check_view(a.vp, "V_prefix", 1, a.Hkv, a.P, a.d, 2, &svp)) != BF_OK) return rc;
+    }
+    if (a.P > 0 && !plan.together) {
         if ((rc = bind_context()) != BF_OK) return rc;
         PrefixArgs x;
         memset(&x, 0, sizeof(x));
@@ -635,15 +666,26 @@ int decode_step(const StepArgs& a) {
         x.stream = a.stream;
         if ((rc = bf_prefix_partial(x)) != BF_OK) return rc;
     }
-    if (a.C > 0) {
+    if (a.C > 0 || plan.together) {
         bfk::dec::Params p;
         memset(&p, 0, sizeof(p));
         p.q = a.q;
-        p.k = reinterpret_cast<const char*>(a.k->data);
-        p.v = reinterpret_cast<const char*>(a.v->data);
-        for (int i = 0; i < 3; ++i) {
-            p.ks[i] = sk.s[i] * 2;
-            p.vs[i] = sv.s[i] * 2;
+        if (a.C > 0) {
+            p.k = reinterpret_cast<const char*>(a.k->data);
+            p.v = reinterpret_cast<const char*>(a.v->data);
+            for (int i = 0; i < 3; ++i) {
+                p.ks[i] = sk.s[i] * 2;
+                p.vs[i] = sv.s[i] * 2;
+            }
+        }
+        if (plan.together) {
+            p.kp = reinterpret_cast<const char*>(a.kp->data);
+            p.vp = reinterpret_cast<const char*>(a.vp->data);
+            for (int i = 0; i < 2; ++i) {
+                p.kps[i] = skp.s[i + 1] * 2;
+                p.vps[i] = svp.s[i + 1] * 2;
+            }
+            p.prefix = a.P;
         }
         p.lengths = a.lengths;
         p.out = a.o;
@@ -659,15 +701,16 @@ int decode_step(const StepArgs& a) {
         p.window = a.window < a.C ? a.window : a.C;
         p.sinks = a.sinks < a.C ? a.sinks : a.C;
         p.chunk = plan.chunk;
-        p.beside = a.P > 0;
+        p.beside = a.P > 0 && !plan.together;
         p.scale_log2 = a.scale * kLog2e;
         const long long units = (long long)a.B * a.Hkv * plan.row_tiles;
-        if (a.d == 64)
-            rc = f16 ? launch_decode<64, true>(p, plan.splits, units, a.stream)
-                     : launch_decode<64, false>(p, plan.splits, units, a.stream);
-        else
-            rc = f16 ? launch_decode<128, true>(p, plan.splits, units, a.stream)
-                     : launch_decode<128, false>(p, plan.splits, units, a.stream);
+        using Launch = int (*)(const bfk::dec::Params&, int, long long, cudaStream_t);
+        const Launch launch[2][2][2] = {  // [d == 128][fp16][prefix among the keys]
+            {{launch_decode<64, false, false>, launch_decode<64, false, true>},
+             {launch_decode<64, true, false>, launch_decode<64, true, true>}},
+            {{launch_decode<128, false, false>, launch_decode<128, false, true>},
+             {launch_decode<128, true, false>, launch_decode<128, true, true>}}};
+        rc = launch[a.d == 128][f16][plan.together](p, plan.splits, units, a.stream);
         if (rc != BF_OK || plan.direct) return rc;
     }
     bfk::dec::CombineParams c;

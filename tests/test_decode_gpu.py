@@ -130,6 +130,32 @@ def test_prefix_decode_parity(d, ty, b, hq, hkv, t, prefix, cap):
     check_prefix(q, k, v, kp, vp, lengths)
 
 
+@pytest.mark.parametrize("d,ty", [(64, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("b,hq,hkv,t,prefix", [
+    (1, 1, 1, 1, 1), (4, 8, 2, 1, 1000), (33, 8, 2, 1, 129), (5, 10, 2, 1, 300), (70, 4, 1, 3, 257),
+    (2, 16, 1, 9, 200), (3, 6, 3, 1, 5000), (130, 4, 4, 1, 128),
+])
+def test_prefix_decode_large_caches(d, ty, b, hq, hkv, t, prefix):
+    """Capacities for which the prefix is read by a kernel of its own, whatever the lengths are."""
+    cap = (33 << 20) // (b * hkv * ((hq // hkv * t + 15) // 16) * d * 4) + 1
+    q, k, v, kp, vp = make(b, hq, hkv, t, cap, d, ty, seed=b + prefix, prefix=prefix)
+    lengths = torch.randint(0, 60, (b,), device="cuda", dtype=torch.int32,
+                            generator=torch.Generator(device="cuda").manual_seed(b))
+    check_prefix(q, k, v, kp, vp, lengths)
+
+
+@pytest.mark.parametrize("t", [1, 4])
+def test_prefix_decode_sides_of_the_rule(t):
+    """The same step just below and just above the size from which the prefix has its own kernel."""
+    from blackflash_b200 import prefix_decode
+    below = (32 << 20) // (4 * 2 * 128 * 4) - 900
+    q, k, v, kp, vp = make(4, 8, 2, t, below + 1, 128, seed=t, prefix=900)
+    n = lens(0, 2, 1000, below)
+    for cap in (below, below + 1):
+        o64, _, pv = ref.decode_ref(q, k[:, :, :cap], v[:, :, :cap], n, 1 << 40, 0, 1 / math.sqrt(128), kp, vp)
+        ref.check_o(prefix_decode(q, kp, vp, k[:, :, :cap], v[:, :, :cap], n), o64, pv)
+
+
 def test_prefix_decode_without_prefix_or_cache():
     from blackflash_b200 import prefix_decode, window_decode
     q, k, v, kp, vp = make(3, 4, 2, 2, 50, 64, seed=1, prefix=77)
