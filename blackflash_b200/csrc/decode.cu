@@ -10,7 +10,8 @@
 // past a sequence's length are filled with zeros in shared memory and never read from
 // memory, so what a cache holds there (infinities, NaN, addresses past its end) does not
 // matter. The visible keys of a row tile are [0, s0) and [lo, hi); they are numbered
-// through, so that sinks cost no extra pass, and split into chunks over blocks. Chunks
+// through, so that sinks cost no extra pass (nor a short shared prefix, whose keys then come
+// first), and split into chunks over blocks. Chunks
 // leave fp32 partials and their log2-sum-exp2, joined by combine_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,10 +24,11 @@
 namespace bfk {
 namespace dec {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;      // of a block
+constexpr int kWideWarps = 8;  // of a block that has a multiprocessor to itself (Plan::wide)
 constexpr int kStages = 2;  // 64 KiB a block, three blocks a multiprocessor; three stages and two blocks: 3 to 10 % slower
 
-template <int D>
+template <int D, int W>
 struct Cfg {
     static constexpr int kKeys = 2048 / D;          // keys of a warp's step: 4 KiB each of K and V
     static constexpr int kRow = D * 2;              // bytes of a row
@@ -34,7 +36,7 @@ struct Cfg {
     static constexpr int kHalf = kKeys * kRow;      // K (or V) bytes of a stage
     static constexpr int kStage = 2 * kHalf;
     static constexpr int kWarpBytes = kStages * kStage;
-    static constexpr int kSmem = kWarps * kWarpBytes;
+    static constexpr int kSmem = W * kWarpBytes;
     static_assert(kWarpBytes >= 16 * (D + 4) * 4, "the join reuses a warp's stages");
 };
 
@@ -103,9 +105,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // kPrefix: the prefix's keys are the first of the numbering, as sinks are, and every token sees
 // them; each sequence reads them for itself.
-template <int D, bool kF16, bool kPrefix>
-__global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
-    using C = Cfg<D>;
+template <int D, bool kF16, bool kPrefix, int W>
+__global__ void __launch_bounds__(W * 32) decode_kernel(const Params p) {
+    using C = Cfg<D, W>;
     constexpr int NB = C::kKeys / 8;  // score blocks of 8 keys
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -144,11 +146,11 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     const char* kpb = kPrefix ? p.kp + kvh * p.kps[0] : nullptr;
     const char* vpb = kPrefix ? p.vp + kvh * p.vps[0] : nullptr;
     const int groups = (v1 - v0 + C::kKeys - 1) / C::kKeys;
-    const int steps = groups > warp ? (groups - warp + kWarps - 1) / kWarps : 0;
+    const int steps = groups > warp ? (groups - warp + W - 1) / W : 0;
 
     auto load = [&](int s) {
         if (s < steps) {
-            const int vg = v0 + (warp + s * kWarps) * C::kKeys;
+            const int vg = v0 + (warp + s * W) * C::kKeys;
             const uint32_t dst = mine_a + (uint32_t)(s % kStages) * C::kStage;
 #pragma unroll
             for (int i = 0; i < C::kHalf / 512; ++i) {
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
         }
         // Mask and scale. A group of window keys up to the first token's position and inside the
         // last one's window, or of sinks, is visible to every row.
-        const int vg = v0 + (warp + s * kWarps) * C::kKeys;
+        const int vg = v0 + (warp + s * W) * C::kKeys;
         const int k0 = lo + (vg - s0), k1 = k0 + C::kKeys - 1;
         const bool whole = vg + C::kKeys <= v1 &&
                            (vg >= s0 ? k1 <= pos0 && len - 1 - k0 < p.window : vg + C::kKeys <= s0);
@@ -298,13 +300,13 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     cp_async_wait<0>();
     __syncwarp();
 
-    // ---- join of the four warps, in the space of their stages
+    // ---- join of the warps, in the space of their stages
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     constexpr int kPitch = D + 4;  // floats; the four extra spread the rows over the banks
-    __shared__ float sm_m[kWarps][16], sm_l[kWarps][16];
+    __shared__ float sm_m[W][16], sm_l[W][16];
     float* o = reinterpret_cast<float*>(mine);
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
@@ -320,14 +322,14 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Params p) {
     }
     __syncthreads();
     const int rows = min(16, p.q_rows - rt * 16);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kWarps * 32) {
+    for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
         float m = sm_m[0][r];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sm_m[w][r]);
+        for (int w = 1; w < W; ++w) m = fmaxf(m, sm_m[w][r]);
         float l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             // All keys masked: the sum is an exact zero (and not NaN, as of a row of NaN scores).
             if (sm_l[w][r] == 0.f) continue;
             const float f = fast_exp2(sm_m[w][r] - m);
@@ -514,6 +516,7 @@ struct Plan {
     int chunk, splits;    // cache: keys of a split, splits
     int p_splits, p_tiles;  // prefix: splits, KV tiles of a split
     bool together;        // the prefix's keys are read with each sequence's own, by one kernel
+    bool wide;            // blocks of kWideWarps warps
     bool direct;          // one split, no prefix part: the kernel writes O itself
     long long bytes;
 };
@@ -556,13 +559,24 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
         if (i & 1) chunk += chunk / 4;
         chunk = (chunk + 127) / 128 * 128;
         const long long n = (vis + chunk - 1) / chunk, last = vis - (n - 1) * chunk;
-        const long long cost = n * units <= slots ? slots * ((n > 1 ? chunk : vis) + start)
-                                                  : units * (vis + n * start) + slots * (last + start);
+        long long cost = n * units <= slots ? slots * ((n > 1 ? chunk : vis) + start)
+                                            : units * (vis + n * start) + slots * (last + start);
+        if (n > 1) cost += slots * start;  // the join's launch (256 keys at d = 64: 4.1 -> 3.4 us)
         if (best < 0 || cost < best) {
             best = cost;
             p.chunk = (int)chunk;
             p.splits = (int)n;
         }
+    }
+    // Few keys: one block of eight warps a unit and no join, for as many steps a warp as the
+    // units leave multiprocessors idle. us in a graph, wide / split, by units and keys at d = 128:
+    // 8 units, 516 keys 7.2 / 5.7; 64 units, 384 6.0 / 6.9 and 516 7.7 / 7.5; 128 units, 1000 11.4 / 12.5
+    // (wide is one launch instead of two besides, 3 us of the host's).
+    const long long keys = 2048 / d, steps = (vis + bfk::dec::kWideWarps * keys - 1) / (bfk::dec::kWideWarps * keys);
+    p.wide = units <= kPlanSms && vis > bfk::dec::kWarps * keys && steps <= (units > 48 ? units / 16 : 3);
+    if (p.wide) {
+        p.splits = 1;
+        p.chunk = (int)vis;
     }
     p.p_splits = p.p_tiles = 0;
     if (P > 0 && !p.together) {
@@ -596,14 +610,20 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
     return BF_OK;
 }
 
-template <int D, bool kF16, bool kPrefix>
-int launch_decode(const bfk::dec::Params& p, int splits, long long units, cudaStream_t stream) {
+template <int D, bool kF16, bool kPrefix, int W>
+int launch_warps(const bfk::dec::Params& p, int splits, long long units, cudaStream_t stream) {
     static std::atomic<bool> done[64];  // per device; zero-initialised (static storage)
     int rc;
-    auto kernel = bfk::dec::decode_kernel<D, kF16, kPrefix>;
-    if ((rc = allow_smem(kernel, bfk::dec::Cfg<D>::kSmem, done)) != BF_OK) return rc;
-    return launch_error(launch_pdl(kernel, dim3((unsigned)units, (unsigned)splits), bfk::dec::kWarps * 32,
-                                   bfk::dec::Cfg<D>::kSmem, stream, p));
+    auto kernel = bfk::dec::decode_kernel<D, kF16, kPrefix, W>;
+    constexpr int smem = bfk::dec::Cfg<D, W>::kSmem;
+    if ((rc = allow_smem(kernel, smem, done)) != BF_OK) return rc;
+    return launch_error(launch_pdl(kernel, dim3((unsigned)units, (unsigned)splits), W * 32, smem, stream, p));
+}
+
+template <int D, bool kF16, bool kPrefix>
+int launch_decode(const bfk::dec::Params& p, const Plan& plan, long long units, cudaStream_t stream) {
+    return plan.wide ? launch_warps<D, kF16, kPrefix, bfk::dec::kWideWarps>(p, plan.splits, units, stream)
+                     : launch_warps<D, kF16, kPrefix, bfk::dec::kWarps>(p, plan.splits, units, stream);
 }
 
 struct StepArgs {
@@ -704,13 +724,13 @@ int decode_step(const StepArgs& a) {
         p.beside = a.P > 0 && !plan.together;
         p.scale_log2 = a.scale * kLog2e;
         const long long units = (long long)a.B * a.Hkv * plan.row_tiles;
-        using Launch = int (*)(const bfk::dec::Params&, int, long long, cudaStream_t);
+        using Launch = int (*)(const bfk::dec::Params&, const Plan&, long long, cudaStream_t);
         const Launch launch[2][2][2] = {  // [d == 128][fp16][prefix among the keys]
             {{launch_decode<64, false, false>, launch_decode<64, false, true>},
              {launch_decode<64, true, false>, launch_decode<64, true, true>}},
             {{launch_decode<128, false, false>, launch_decode<128, false, true>},
              {launch_decode<128, true, false>, launch_decode<128, true, true>}}};
-        rc = launch[a.d == 128][f16][plan.together](p, plan.splits, units, a.stream);
+        rc = launch[a.d == 128][f16][plan.together](p, plan, units, a.stream);
         if (rc != BF_OK || plan.direct) return rc;
     }
     bfk::dec::CombineParams c;

@@ -104,8 +104,8 @@ def prefix_decode(Q: torch.Tensor, K_prefix: torch.Tensor, V_prefix: torch.Tenso
                   V_cache: torch.Tensor, lengths: torch.Tensor, scale: float | None = None, want_lse: bool = False):
     """The step of T new tokens a sequence, Q [B, Hq, T, d], for a batch behind one prefix.
 
-    K_prefix, V_prefix [Hkv, P, d] are shared by all sequences and are read once for the
-    whole batch; K_cache, V_cache [B, Hkv, C, d] hold what each sequence has of its own,
+    K_prefix, V_prefix [Hkv, P, d] are shared by all sequences, and a long one is read
+    once for the whole batch; K_cache, V_cache [B, Hkv, C, d] hold what each sequence has of its own,
     lengths [B] int32 of it, the T new tokens among them. New token t of sequence b sees the
     whole prefix and the keys j <= lengths[b] - T + t of its own cache. P or C may be 0.
     Returns O [B, Hq, T, d], or (O, lse) with want_lse; a token that sees no key gets 0 and

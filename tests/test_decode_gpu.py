@@ -206,3 +206,18 @@ def test_steps_on_other_streams_and_in_two_graphs():
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("d,ty", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("b,hq,hkv,t,cap,window,sinks", [
+    (1, 8, 2, 1, 130, 999, 0), (1, 8, 2, 1, 384, 100, 6), (1, 8, 2, 1, 385, 999, 0), (1, 8, 2, 1, 769, 999, 0),
+    (2, 6, 3, 7, 700, 300, 5), (37, 4, 4, 1, 1100, 1024, 4), (37, 8, 4, 1, 1025, 9999, 0), (149, 1, 1, 2, 384, 380, 1),
+    (13, 6, 6, 1, 513, 257, 1),
+])
+def test_decode_few_keys(d, ty, b, hq, hkv, t, cap, window, sinks):
+    """Around the sizes up to which one block, of four warps or of eight, takes all keys of a head."""
+    q, k, v = make(b, hq, hkv, t, cap, d, ty, seed=cap)
+    lengths = torch.randint(0, cap + 1, (b,), device="cuda", dtype=torch.int32,
+                            generator=torch.Generator(device="cuda").manual_seed(b))
+    lengths[-1] = cap
+    check_window(q, k, v, lengths, window, sinks)

@@ -83,7 +83,8 @@ def test_views_are_checked(lib, bad, text):
 def test_decode_plans_and_refusals(lib):
     ws = lib.blackflash_decode_workspace_bytes
     assert ws(1, 8, 2, 1, 0, 64, 64, 64, 0) == 0          # one split: no workspace
-    assert ws(1, 8, 2, 1, 0, 100000, 64, 512, 4) > 0
+    assert ws(1, 8, 2, 1, 0, 100000, 64, 512, 4) == 0     # few keys: one block each
+    assert ws(1, 8, 2, 1, 0, 100000, 64, 5000, 4) > 0
     # The plan follows the window, not the capacity.
     assert ws(1, 8, 2, 1, 0, 1 << 30, 128, 512, 4) == ws(1, 8, 2, 1, 0, 1000, 128, 512, 4)
     assert ws(64, 32, 8, 1, 16384, 1024, 128, 2 ** 31 - 1, 0) % 4 == 0
