@@ -102,7 +102,7 @@ def test_decode_plans_and_refusals(lib):
         assert lib.blackflash_window_decode(*args, *sizes) == 1
         assert text in lib.blackflash_last_error()
     big = 1 << 30
-    p = (1, 8, 2, 1, 100, 50, 64)
+    p = (1, 8, 2, 1, 9000, 50, 64)  # enough keys to be split: with a workspace
     for args, text in (((16, None, v, v, v, 16, 16, None, 32, big), b"prefix"), ((16, v, v, v, None, 16, 16, None, 32, big), b"V_cache"),
                        ((16, v, v, v, v, 16, 16, None, None, big), b"workspace")):
         assert lib.blackflash_prefix_decode(*args, *p, 0.125, 0, None) == 1
