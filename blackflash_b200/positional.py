@@ -151,9 +151,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
         def index_of(turns: float) -> float:  # of the pair that turns that often within original_length
             return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        lo = max(math.floor(index_of(beta_fast)), 0)
-        hi = min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
-        ramp = ((pair - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        # Not held to the pairs that exist: either end may lie beyond the first or the last one.
+        lo, hi = math.floor(index_of(beta_fast)), math.ceil(index_of(beta_slow))
+        ramp = ((pair - lo) / max(hi - lo, 1)).clamp(0, 1)
         freqs = freqs * (1 - ramp) + freqs / factor * ramp
         amplitude = 0.1 * math.log(factor) + 1.0
     return freqs.to(device if device is not None else "cuda"), amplitude

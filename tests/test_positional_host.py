@@ -156,3 +156,31 @@ def test_rotary_frequency_scalings():
     g, a = rotary_frequencies(64, 10000.0, "by-parts", 8.0, 4096, device="cpu")
     assert torch.equal(g[:5], f[:5]) and torch.allclose(g[-5:], f[-5:] / 8, rtol=1e-14, atol=0)
     assert (g[1:] < g[:-1]).all() and abs(a - (1 + 0.1 * math.log(8))) < 1e-15
+
+
+@pytest.mark.parametrize("rot,base,length,fast,slow", [
+    (64, 1e4, 100, 64.0, 32.0),    # every pair turns less than beta_slow times: the fastest 15.9
+    (64, 1e4, 4, 32.0, 1.0),       # 0.64 turns
+    (64, 1e4, 150, 32.0, 1.0),     # the fastest pair (23.9 turns) lies inside the ramp
+    (32, 1e4, 1 << 24, 32.0, 1.0),  # every pair turns more than beta_fast times: the slowest 475
+    (16, 100.0, 4096, 32.0, 8.0),  # the slowest pair (11.6 turns) lies inside the ramp
+    (2, 1e4, 4096, 32.0, 1.0), (128, 5e5, 8192, 32.0, 1.0),
+])
+def test_by_parts_follows_the_turns_of_each_pair(rot, base, length, fast, slow):
+    """Pairs above beta_fast turns stay, those below beta_slow are divided by the factor, and
+    between them the share of the divided frequency rises by equal steps."""
+    from blackflash_b200 import rotary_frequencies
+    factor = 8.0
+    f = rotary_frequencies(rot, base, device="cpu")[0]
+    g = rotary_frequencies(rot, base, "by-parts", factor, length, fast, slow, device="cpu")[0]
+    turns = length * f / (2 * math.pi)
+    share = (1 - g / f) / (1 - 1 / factor)  # 0: kept, 1: divided; fp64 rounding alone is off
+    assert (share[turns > fast].abs() < 1e-12).all() and ((share[turns < slow] - 1).abs() < 1e-12).all()
+    assert ((share > -1e-12) & (share < 1 + 1e-12)).all()
+    inside = (share > 1e-9) & (share < 1 - 1e-9)
+    steps = share[inside].diff()
+    assert (steps > 0).all() and (steps.numel() < 2 or (steps - steps[0]).abs().max() < 1e-12)
+    # The ramp spans the whole pairs around the two bounds, so its step is known.
+    ends = [rot * math.log(length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (fast, slow)]
+    if steps.numel():
+        assert abs(steps[0] * (math.ceil(ends[1]) - math.floor(ends[0])) - 1) < 1e-9
