@@ -530,17 +530,17 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
     if (window < 1 || sinks < 0) return bf_set_error(BF_ERR_ARG, "need window >= 1 and sinks >= 0");
     Plan& p = *out;
     const long long q_rows = (long long)(Hq / Hkv) * T;
+    // Checked by division: three factors of 31 bits pass 64, and `units` below is a divisor.
+    if (q_rows > (1 << 20) || (long long)B * Hq > 0x7fffffffLL / T) return bf_set_error(BF_ERR_ARG, "too many query rows");
     p.rows = (long long)B * Hq * T;
-    if (q_rows > (1 << 20) || p.rows > 0x7fffffffLL) return bf_set_error(BF_ERR_ARG, "too many query rows");
     p.row_tiles = (int)((q_rows + 15) / 16);
     const long long units = (long long)B * Hkv * p.row_tiles;
-    if (units > 0x7fffffffLL) return bf_set_error(BF_ERR_ARG, "too many query rows");
     // The longest run of keys a row tile can see.
     long long vis = (long long)window + T - 1 + sinks;
     if (vis > C) vis = C;
     // A short prefix is not worth a kernel of its own, which reads it once for the batch but
     // takes a launch, its start and parts to join.
-    p.together = P > 0 && units * (P + vis) * d * 4 <= kTogetherBytes;
+    p.together = P > 0 && P + vis <= kTogetherBytes / (d * 4) / units;
     if (p.together) vis += P;
     // Splits: blocks run three a multiprocessor, a unit's splits one grid row after the other, so
     // that the last, shorter ones fill up what the others leave. The time of a chunk size, in
@@ -589,14 +589,14 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
         // ends first, in ns as measured: a step of two 128-row tiles, a block's start and end,
         // the bytes a multiprocessor streams (the caches half full), a part's write and read.
         const long long step = d == 128 ? 2200 : 1300, ends = 5000;
-        const long long cache = (long long)B * Hkv * C * d * 2 / 50;  // ns of one multiprocessor
+        const double cache = floor((double)B * Hkv * C * d * 2 / 50);  // ns of one multiprocessor
         best = -1;
         for (int n = 1; n <= nk && n <= 2 * kPlanSms; n += 1 + n / 16) {
             const int s = (nk + n - 1) / n, real = (nk + s - 1) / s;
             const long long blocks = real * u, used = blocks < kPlanSms ? blocks : kPlanSms;
             const long long t = (blocks + kPlanSms - 1) / kPlanSms * (s * step + ends);
-            const long long meanwhile = (kPlanSms - used) * t;
-            const long long after = cache > meanwhile ? (cache - meanwhile) / kPlanSms : 0;
+            const double meanwhile = (double)((kPlanSms - used) * t);
+            const long long after = cache > meanwhile ? (long long)((cache - meanwhile) / kPlanSms) : 0;
             const long long cost = t + after + real * p.rows * d * 8 / 3000;
             if (best < 0 || cost < best) {
                 best = cost;

@@ -167,6 +167,22 @@ BwdPlan bwd_plan(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int
     return p;
 }
 
+// The sizes of the backward and its plan. The limits of a launch come before the plan: within
+// them its products fit 64 bits.
+int check_bwd(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale, BwdPlan* plan) {
+    int rc;
+    if ((rc = check_window(B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale)) != BF_OK) return rc;
+    const long long heads = (long long)B * Hq, n_pad = (Nq + 127) / 128 * 128;
+    bool fits = heads <= 0x7fffffffLL && heads * n_pad / 8 <= 0x7fffffffLL &&
+                (Hq / Hkv) * (n_pad / bfk::winb::NT) <= 0x7fffffffLL;
+    if (fits) {
+        *plan = bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks);
+        const long long parts = (long long)plan->ns * plan->splits_s + (long long)(plan->nk - plan->ns) * plan->splits_n;
+        fits = parts <= 0x7fffffffLL / ((long long)B * Hkv);
+    }
+    return fits ? BF_OK : bf_set_error(BF_ERR_ARG, "problem too large for one launch");
+}
+
 // `first`: dK/dV items of sink tiles, which come first, and how many times the others' length they
 // have. Blocks that begin with one of them take so many items less of the others: with all in
 // turn, 32 blocks at B=2 H=16 N=4096 window 1024 had 172 steps where the mean is 134 (the
@@ -209,8 +225,8 @@ int launch_bwd(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& 
 extern "C" long long blackflash_window_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nkv, int d, int window,
                                                            int sinks) {
     bf_set_error(BF_OK, "");
-    if (check_window(B, Hq, Hkv, Nq, Nkv, d, window, sinks, 1.f) != BF_OK) return -1;
-    return bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks).bytes;
+    BwdPlan plan;
+    return check_bwd(B, Hq, Hkv, Nq, Nkv, d, window, sinks, 1.f, &plan) == BF_OK ? plan.bytes : -1;
 }
 
 extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, const void* O, const bf_view* dO,
@@ -219,7 +235,8 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
                                      int sinks, float scale, void* stream) {
     bf_set_error(BF_OK, "");
     int rc;
-    if ((rc = check_window(B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale)) != BF_OK) return rc;
+    BwdPlan plan;
+    if ((rc = check_bwd(B, Hq, Hkv, Nq, Nkv, d, window, sinks, scale, &plan)) != BF_OK) return rc;
     ViewStrides sq, sk, sv, sd;
     if ((rc = check_view(Q, "Q", B, Hq, Nq, d, 2, &sq)) != BF_OK) return rc;
     if ((rc = check_view(K, "K", B, Hkv, Nkv, d, 2, &sk)) != BF_OK) return rc;
@@ -230,7 +247,6 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
         if (!ptr || (reinterpret_cast<uintptr_t>(ptr) & 31u))
             return bf_set_error(BF_ERR_ARG, "O, dQ, dK, dV and the workspace must be non-null and 32-byte aligned");
     if (!lse) return bf_set_error(BF_ERR_ARG, "lse: null pointer");
-    const BwdPlan plan = bwd_plan(B, Hq, Hkv, Nq, Nkv, d, window, sinks);
     if (workspace_bytes < plan.bytes)
         return bf_set_error(BF_ERR_ARG, "workspace smaller than blackflash_window_bwd_workspace_bytes()");
     const int nt = bfk::winb::NT;
@@ -238,9 +254,6 @@ extern "C" int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const b
     const long long units = (long long)B * Hkv;
     const long long kv_items = units * ((long long)plan.ns * plan.splits_s + (long long)(plan.nk - plan.ns) * plan.splits_n);
     const long long q_items = (long long)B * Hq * q_tiles;
-    if ((long long)B * Hq > 0x7fffffffLL || kv_items > 0x7fffffffLL || q_items > 0x7fffffffLL ||
-        (long long)(Hq / Hkv) * (plan.n_pad / nt) > 0x7fffffffLL || plan.vec / 8 > 0x7fffffffLL)
-        return bf_set_error(BF_ERR_ARG, "problem too large for one launch");
 
     if ((rc = bind_context()) != BF_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -184,3 +184,37 @@ def test_by_parts_follows_the_turns_of_each_pair(rot, base, length, fast, slow):
     ends = [rot * math.log(length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (fast, slow)]
     if steps.numel():
         assert abs(steps[0] * (math.ceil(ends[1]) - math.floor(ends[0])) - 1) < 1e-9
+
+
+HUGE_SIZES = """
+from blackflash_b200 import _lib
+lib = _lib.load()
+def refused(x):
+    assert x == -1 and lib.blackflash_last_error(), x
+big = 1 << 30
+for b, hq, hkv, t in ((big, big, big, 256), (big, big, big, 16), (big, big, big, 1), (1 << 16, 1 << 16, 1 << 16, 1 << 20),
+                      (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 1), (1 << 11, 1 << 10, 1 << 10, 1 << 10)):
+    for p, c in ((0, 64), (big, 0), (big, big)):
+        refused(lib.blackflash_decode_workspace_bytes(b, hq, hkv, t, p, c, 64, 4, 0))
+# The most rows, and the most keys, that are taken.
+assert lib.blackflash_decode_workspace_bytes(2 ** 31 - 1, 1, 1, 1, big, big, 128, 2 ** 31 - 1, 2 ** 31 - 1) > 0
+assert lib.blackflash_decode_workspace_bytes(1 << 20, 1 << 10, 1 << 10, 1, big, big, 128, 2 ** 31 - 1, 0) > 0
+for b, hq, hkv, nq, nkv, w, s in ((big, big, big, big, big, 4, 0), (1 << 16, 1 << 16, 1 << 16, big, 1, 4, 0),
+                                  (1 << 20, 1 << 20, 1, big, big, big, big), (1 << 16, 1, 1, big, 1, 4, 0),
+                                  (1 << 20, 1, 1, 1, big, 4, 0)):
+    refused(lib.blackflash_window_bwd_workspace_bytes(b, hq, hkv, nq, nkv, 64, w, s))
+assert lib.blackflash_window_bwd_workspace_bytes(1, 8, 8, big, big, 64, big, big) >= 4 * 6 * 8 * big
+assert lib.blackflash_window_bwd_workspace_bytes(1, 1, 1, 1, big, 128, big, big) > 0
+print("refused")
+"""
+
+
+def test_sizes_whose_products_pass_64_bits():
+    """Refused, not divided by: in a process of its own, which a division by zero would end."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", HUGE_SIZES], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "refused" in out.stdout, (out.returncode, out.stderr[-2000:])
