@@ -485,6 +485,18 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     return d;
 }
 
+// Maxima that are NaN if any argument is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 2^x for a pair of arguments on the FMA pipe instead of MUFU.
 // Range reduction 2^x = 2^n * 2^f, n = rint(x), f = x - n in [-1/2, 1/2]; 2^f by a
 // degree-3 polynomial with minimax relative error 7.5e-5 (coefficients from

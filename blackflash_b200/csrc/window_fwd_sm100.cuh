@@ -370,17 +370,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
-                    mx0 = fmax3(mx0, __uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1]));
-                    mx1 = fmax3(mx1, __uint_as_float(s[1][c]), __uint_as_float(s[1][c + 1]));
+                    mx0 = fmax3_nan(mx0, __uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1]));
+                    mx1 = fmax3_nan(mx1, __uint_as_float(s[1][c]), __uint_as_float(s[1][c + 1]));
                 }
-                float mx = fmaxf(mx0, mx1);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                float mx = fmax_nan(mx0, mx1);
+                mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                 const float m_new = mx * p.scale_log2;
                 // Lazy rescale: keep the old maximum unless the tile's exceeds it by more than
                 // 8 (log2 units). A row that has seen nothing yet refers to 0, so that its
-                // masked scores give 2^-inf and not NaN.
+                // masked scores give 2^-inf and not NaN. A NaN score makes the row's maximum NaN and
+                // so, through alpha, its sum, whichever columns the FMA-pipe exponential takes (it
+                // has no NaN of its own); the comparison is written for that.
                 float alpha = 1.f;
-                const bool need = m_new > m_use + 8.0f;
+                const bool need = !(m_new <= m_use + 8.0f);
                 if (need) {
                     alpha = fast_exp2(m_use - m_new);
                     m_use = m_new;
@@ -453,7 +455,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(bar_pv, (g - 1) & 1u, ctl, kSiteSoftPV))) break;
                 tc_fence_after();
             }
-            const float l_sum = l_half + __shfl_xor_sync(0xffffffffu, l_half, 16);
+            float l_sum = l_half + __shfl_xor_sync(0xffffffffu, l_half, 16);
+            // A score of +inf stays the maximum, and its weight is 2^(inf - inf): the row is NaN.
+            if (m_use == INFINITY) l_sum = NAN;
             const bool empty = m_use == -INFINITY && l_sum == l_sum;  // a row of NaN scores is not empty
             const float inv = empty ? 0.f : 1.f / l_sum;
             const float lse2 = empty ? -INFINITY : m_use - kShift + __log2f(l_sum);

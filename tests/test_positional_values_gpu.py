@@ -1,0 +1,88 @@
+"""Position-aware operators on values at the edge of their types, against fp64."""
+import math
+
+import pytest
+import torch
+
+import positional_ref as ref
+from test_window_gpu import make
+
+pytestmark = pytest.mark.gpu
+
+
+def same_outside(got, want, rows):
+    """Rows in `rows` are NaN in every column, all others as they were, bit for bit."""
+    assert torch.isnan(got[rows]).all(), f"{int((~torch.isnan(got[rows])).sum())} numbers where a row sees a NaN"
+    assert torch.equal(got[~rows], want[~rows])
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (3, 3)])
+@pytest.mark.parametrize("base,sinks", [(0, 4), (64, 0), (130, 130), (184, 40)])
+def test_a_key_of_nan_reaches_the_rows_that_see_it(t, d, hq, hkv, base, sinks):
+    """At every index of 16: none may hide in columns that another form of the exponential takes."""
+    from blackflash_b200 import window_attention_lse
+    n, window = 200, 60
+    q, k, v = make(16, hq, hkv, n, n, d, t, seed=base)
+    want, want_lse = window_attention_lse(q, k, v, window, sinks)
+    seen = ref.visible(n, n, window, sinks, "cuda")
+    rows = torch.zeros(16, hq, n, dtype=torch.bool, device="cuda")
+    for i in range(16):
+        k[i, -1, base + i] = math.nan  # of the last KV head
+        rows[i, -(hq // hkv):] = seen[:, base + i]
+    got, lse = window_attention_lse(q, k, v, window, sinks)
+    same_outside(got, want, rows)
+    same_outside(lse, want_lse, rows)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sinks", [0, 100])
+def test_infinite_scores(t, d, sinks):
+    """A score of +inf (or of inf times 0) makes its row NaN, as the definition does; one of -inf
+    has weight 0."""
+    from blackflash_b200 import window_attention_lse
+    n, window, base = 300, 90, 64
+    q, k, v = make(16, 2, 2, n, n, d, t, seed=7)
+    seen = ref.visible(n, n, window, sinks, "cuda").repeat(16, 2, 1, 1)
+    rows = torch.zeros(16, 2, n, dtype=torch.bool, device="cuda")
+    for i in range(16):
+        rows[i] = seen[i, :, :, base + i] & (q[i, :, :, 5] >= 0)
+        k[i, :, base + i, 5] = 0  # for the statement, which leaves that key out
+        seen[i, :, :, base + i] = False
+    o64, lse64, _, pv = ref.attention64(q.double(), k.double(), v.double(), seen, 1 / math.sqrt(d))
+    for i in range(16):
+        k[i, :, base + i, 5] = math.inf
+    got, lse = window_attention_lse(q, k, v, window, sinks)
+    assert torch.isnan(got[rows]).all() and torch.isnan(lse[rows]).all()
+    ref.check_o(got[~rows], o64[~rows], pv[~rows])
+    ref.check_lse(lse[~rows], lse64[~rows])
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_prefix_key_of_nan_reaches_every_row(t, d):
+    """In the prefix's own kernel (a large cache, hardly used), at every index of 16."""
+    from blackflash_b200 import prefix_decode, wait_status
+    b, hq, hkv, p = 4, 8, 2, 300
+    cap = (33 << 20) // (b * hkv * d * 4) + 1
+    gen = torch.Generator(device="cuda").manual_seed(d)
+
+    def rnd(*s):
+        return torch.randn(s, generator=gen, device="cuda").to(t)
+    q, kp, vp = rnd(b, hq, 1, d), rnd(hkv, p, d), rnd(hkv, p, d)
+    k, v = torch.zeros(2, b, hkv, cap, d, dtype=t, device="cuda")
+    k[:, :, :9], v[:, :, :9] = rnd(b, hkv, 9, d), rnd(b, hkv, 9, d)
+    n = torch.tensor([0, 1, 9, 4], dtype=torch.int32, device="cuda")
+    want, want_lse = prefix_decode(q, kp, vp, k, v, n, want_lse=True)
+    rows = torch.zeros(b, hq, 1, dtype=torch.bool, device="cuda")
+    rows[:, hq // hkv:] = True
+    for key in range(140, 156):
+        bad = kp.clone()
+        bad[1, key] = math.nan
+        got, lse = prefix_decode(q, bad, vp, k, v, n, want_lse=True)
+        same_outside(got, want, rows)
+        same_outside(lse, want_lse, rows)
+    torch.cuda.synchronize()
+    assert wait_status() == 0
