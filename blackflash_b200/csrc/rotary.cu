@@ -53,6 +53,11 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// The turn, its fused products written out: left to the compiler, they were fused the one way or
+// the other by vector width, and a view's alignment showed in the last bit.
+__device__ __forceinline__ float turn_u(float u, float w, float2 cs) { return fmaf(u, cs.x, -__fmul_rn(w, cs.y)); }
+__device__ __forceinline__ float turn_w(float u, float w, float2 cs) { return fmaf(u, cs.y, __fmul_rn(w, cs.x)); }
+
 template <typename T, int V>
 struct __align__(sizeof(T) * V) Vec {
     T e[V];
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(kBlock, 8) rotary_kernel(const Params p) {
         sincospif(hi, &s, &co);
         // First-order step for what the cast to fp32 dropped (up to 2^-24 of the angle).
         const float lo = (float)(angle - (double)hi) * 3.14159265f;
-        cs[i] = make_float2((co - s * lo) * p.amplitude, (s + co * lo) * p.amplitude * p.sign);
+        cs[i] = make_float2(fmaf(-s, lo, co) * p.amplitude, fmaf(co, lo, s) * p.amplitude * p.sign);
     }
     __syncthreads();
 
@@ -130,8 +135,8 @@ __global__ void __launch_bounds__(kBlock, 8) rotary_kernel(const Params p) {
                     for (int e = 0; e < V; e += 2) {
                         const float2 cw = tab[e >> 1];
                         const float u = to_f<T>(a.e[e]), v = to_f<T>(a.e[e + 1]);
-                        a.e[e] = from_f<T>(u * cw.x - v * cw.y);
-                        a.e[e + 1] = from_f<T>(u * cw.y + v * cw.x);
+                        a.e[e] = from_f<T>(turn_u(u, v, cw));
+                        a.e[e + 1] = from_f<T>(turn_w(u, v, cw));
                     }
                 } else {
                     VT c = *reinterpret_cast<const VT*>(x + half);
@@ -139,8 +144,8 @@ __global__ void __launch_bounds__(kBlock, 8) rotary_kernel(const Params p) {
                     for (int e = 0; e < V; ++e) {
                         const float2 cw = tab[e];
                         const float u = to_f<T>(a.e[e]), v = to_f<T>(c.e[e]);
-                        a.e[e] = from_f<T>(u * cw.x - v * cw.y);
-                        c.e[e] = from_f<T>(u * cw.y + v * cw.x);
+                        a.e[e] = from_f<T>(turn_u(u, v, cw));
+                        c.e[e] = from_f<T>(turn_w(u, v, cw));
                     }
                     *reinterpret_cast<VT*>(y + half) = c;
                 }

@@ -86,3 +86,18 @@ def test_a_prefix_key_of_nan_reaches_every_row(t, d):
         same_outside(lse, want_lse, rows)
     torch.cuda.synchronize()
     assert wait_status() == 0
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_bits_do_not_depend_on_the_alignment(t, interleaved):
+    """A view that starts on a pair and one that starts on 16 bytes give the same bits."""
+    from blackflash_b200 import rotary, rotary_frequencies
+    freqs, amp = rotary_frequencies(128, 500000.0, "by-parts", 4.0, 8192)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, 6, 200, 128, generator=gen, device="cuda").to(t)
+    pos = torch.randint(0, 1 << 20, (2, 200), generator=gen, device="cuda")
+    wide = torch.zeros(2, 6, 200, 136, dtype=t, device="cuda")
+    wide[..., 2:130] = x
+    outs = [rotary(v, v[:, :2], pos, freqs, interleaved, amp) for v in (x, wide[..., 2:130])]
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
