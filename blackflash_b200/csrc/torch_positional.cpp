@@ -9,6 +9,8 @@
 #include <cmath>
 #include <limits>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/blackflash_b200.h"
 
@@ -141,17 +143,33 @@ Tensor rows(const Tensor& t) {
 
 // What a backward refuses. A node keeps the stream that it was made on, a leaf's too while any
 // graph of the leaf lives; the engine would have the default stream wait for a captured one,
-// which ends the capture and, on the engine's thread, the process.
+// which ends the capture and, on the engine's thread, the process. It does so for every node that
+// this backward goes on to, and for no other: behind views and other operations, but not for
+// an input whose gradient was not asked for.
 void check_backward() {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "this operator is differentiable once: its backward does not support create_graph=True");
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
-    const auto node = torch::autograd::get_current_node();
-    for (const auto& edge : node->next_edges()) {
-        const auto stream = edge.function ? edge.function->stream() : c10::nullopt;
-        TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
-                    "a backward cannot be captured while a graph of its inputs from the default stream is alive: drop that "
-                    "graph first, or make it on another stream");
+    const auto* planned = torch::autograd::get_current_graph_task_exec_info();  // empty: every node
+    const auto here = torch::autograd::get_current_node();
+    std::vector<const torch::autograd::Node*> todo{here.get()};
+    std::unordered_set<const torch::autograd::Node*> known;
+    while (!todo.empty()) {
+        const auto* node = todo.back();
+        todo.pop_back();
+        for (const auto& edge : node->next_edges()) {
+            auto* next = edge.function.get();
+            if (!next || !known.insert(next).second) continue;
+            if (planned && !planned->empty()) {
+                const auto plan = planned->find(next);
+                if (plan == planned->end() || !plan->second.should_execute()) continue;
+            }
+            const auto stream = next->stream();
+            TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                        "a backward cannot be captured while a graph of its inputs from the default stream is alive: drop "
+                        "that graph first, or make it on another stream");
+            todo.push_back(next);
+        }
     }
 }
 

@@ -229,6 +229,67 @@ def test_captured_backward_beside_an_eager_graph_of_its_leaves():
     assert out.returncode == 0 and out.stdout.split("\n")[:-1] == lines, out.stdout + out.stderr[-2000:]
 
 
+CAPTURED_PROJECTION = """
+import torch
+import blackflash_b200 as bf
+x = torch.randn(2, 200, 6, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)  # [B, N, H, d]
+w = torch.randn(2, 2, 200, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+freqs, _ = bf.rotary_frequencies(64)
+pos = torch.arange(200, device="cuda")
+grad = torch.ones(2, 4, 200, 64, device="cuda", dtype=torch.bfloat16)
+def window(a=x):
+    h = a.transpose(1, 2)
+    return bf.window_attention_with_grad(h[:, :4], h[:, 4:], h[:, 4:], 50, 4)
+def chain(a=x):
+    q, k = bf.rotary_with_grad(a[:, :, :4].transpose(1, 2), a[:, :, 4:].transpose(1, 2), pos, freqs)
+    return bf.window_attention_with_grad(q, k, k * 2, 50, 4)
+def beside(a=x):
+    return bf.window_attention_with_grad(a[:, :, :4].transpose(1, 2), w, w, 50, 4)
+def warm(step):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+def captured(step):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    return [t.clone() for t in got]
+def check(name, form, leaves, alive):
+    step = lambda: torch.autograd.grad(form(), leaves, grad)
+    warm(step)
+    alive = alive()
+    try:
+        captured(step)
+        print("captured", name, flush=True)
+    except RuntimeError as e:
+        assert "graph of its inputs" in str(e), e
+        print("refused", name, flush=True)
+    del alive
+    assert all(torch.equal(a, b) for a, b in zip(captured(step), step())), name
+    print("alone", name, flush=True)
+check("window", window, [x], lambda: x * 1)
+check("chain", chain, [x], lambda: x * 1)
+# A leaf that this backward does not reach may keep its graph.
+check("beside", beside, [x], lambda: w * 1)
+"""
+
+
+def test_captured_backward_through_other_operations():
+    """The leaf lies behind a transposed view or a slice: refused in words all the same, and only
+    where the backward reaches a leaf whose graph lives."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", CAPTURED_PROJECTION], cwd=root, capture_output=True, text=True, timeout=300)
+    lines = ["refused window", "alone window", "refused chain", "alone chain", "captured beside", "alone beside"]
+    assert out.returncode == 0 and out.stdout.split("\n")[:-1] == lines, out.stdout + out.stderr[-2000:]
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_other_device_than_the_current():
     import blackflash_b200 as bf
