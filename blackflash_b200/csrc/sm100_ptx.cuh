@@ -508,11 +508,18 @@ constexpr float kExp2C0 = 0.9999281167984009f;
 constexpr float kExp2C1 = 0.6932609677314758f;
 constexpr float kExp2C2 = 0.24261054396629333f;
 constexpr float kExp2C3 = 0.05517132207751274f;
+// The other bound: the least argument above -127 for which p(f) is still no less than 1, by a few
+// steps. There p's exponent field and n cancel, and what is left are p's low mantissa bits: 2^-144,
+// which is 0 as bf16 (2^-126 is not, and shows beside a value of 10^38). Weights below 2^-126
+// come out as a smaller number of their size or as 0.
+constexpr float kExp2Zero = -126.99989318847656f;
 
+template <bool kZero = false>
 __device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x2) {
+    constexpr float least = kZero ? kExp2Zero : -126.f;
     float x0, x1;
     f2_unpack(x2, x0, x1);
-    x2 = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    x2 = f2_pack(fmaxf(x0, least), fmaxf(x1, least));
     const uint64_t magic = f2_pack(12582912.f, 12582912.f);  // 1.5 * 2^23: x + magic rounds x to an integer
     const uint64_t t = f2_add(x2, magic);
     const uint64_t n = f2_add(t, f2_pack(-12582912.f, -12582912.f));

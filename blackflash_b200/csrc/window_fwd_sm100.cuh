@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // At d = 64 one pair of eight takes the FMA pipe, as in the dense kernel; at
                         // d = 128 MUFU has headroom.
                         if (D == 64 && ((q * 16 + c) & 7) == 0) {
-                            p2 = exp2_poly_x2(x2);
+                            p2 = exp2_poly_x2<true>(x2);
                         } else {
                             float x0, x1;
                             f2_unpack(x2, x0, x1);

@@ -101,3 +101,38 @@ def test_rotary_bits_do_not_depend_on_the_alignment(t, interleaved):
     wide[..., 2:130] = x
     outs = [rotary(v, v[:, :2], pos, freqs, interleaved, amp) for v in (x, wide[..., 2:130])]
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def largest(shape, t, seed):
+    """Random signs of the type's largest number."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    sign = torch.randint(0, 2, shape, generator=gen, device="cuda") * 2 - 1
+    return (sign * torch.finfo(t).max).to(t)
+
+
+def unseen_keys(t, d, nq, window, sinks):
+    """A chunk of queries, its keys, and which of these no query sees (zero so far)."""
+    n = 256
+    q, k, v = make(2, 4, 2, nq, n, d, t, seed=nq)
+    unseen = ~ref.visible(nq, n, window, sinks, "cuda").any(0)
+    assert unseen.sum() > 50
+    k[:, :, unseen], v[:, :, unseen] = 0, 0
+    return q, k, v, unseen
+
+
+CHUNKS = pytest.mark.parametrize("nq,window,sinks", [(8, 16, 4), (8, 16, 0), (130, 16, 0), (1, 1, 0), (40, 60, 100)])
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@CHUNKS
+def test_masked_keys_of_the_largest_size(t, d, nq, window, sinks):
+    """Finite keys and values that no query sees have weight 0, however large: what a cache may
+    hold between the sinks and the window."""
+    from blackflash_b200 import window_attention_lse
+    q, k, v, unseen = unseen_keys(t, d, nq, window, sinks)
+    o64, lse64, pv = ref.window_ref(q, k, v, window, sinks, 1 / math.sqrt(d))
+    k[:, :, unseen], v[:, :, unseen] = (largest(k[:, :, unseen].shape, t, s) for s in (1, 2))
+    o, lse = window_attention_lse(q, k, v, window, sinks)
+    ref.check_o(o, o64, pv)
+    ref.check_lse(lse, lse64)
