@@ -496,6 +496,11 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 
 // 2^x for a pair of arguments on the FMA pipe instead of MUFU.
 // Range reduction 2^x = 2^n * 2^f, n = rint(x), f = x - n in [-1/2, 1/2]; 2^f by a

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import positional_ref as ref
-from test_window_gpu import make
+from test_window_gpu import check_grads, grads_of, make, upstream
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,41 @@ def test_masked_keys_of_the_largest_size(t, d, nq, window, sinks):
     o, lse = window_attention_lse(q, k, v, window, sinks)
     ref.check_o(o, o64, pv)
     ref.check_lse(lse, lse64)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@CHUNKS
+def test_gradients_beside_masked_keys_of_the_largest_size(d, nq, window, sinks):
+    """dO V^T of such a key passes fp32; its weight is 0 all the same."""
+    q, k, v, unseen = unseen_keys(torch.bfloat16, d, nq, window, sinks)
+    do = upstream(q)
+    plain = (q, k.clone(), v.clone(), do)
+    k[:, :, unseen], v[:, :, unseen] = (largest(k[:, :, unseen].shape, k.dtype, s) for s in (1, 2))
+    check_grads(grads_of(q, k, v, do, window, sinks), *plain, window, sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_upstream_of_rows_that_see_nothing(d):
+    """Queries before the first key have no weight, whatever (finite) gradient comes for them."""
+    q, k, v = make(2, 4, 2, 300, 100, d, seed=3)
+    do = upstream(q)
+    do[:, :, :200] = 0
+    plain = (q, k, v, do.clone())
+    do[:, :, :200] = largest(do[:, :, :200].shape, do.dtype, 3)
+    check_grads(grads_of(q, k, v, do, 30, 2), *plain, 30, 2)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(16, 4), (60, 0), (500, 0)])
+def test_backward_beside_partly_masked_keys_of_the_largest_size(d, window, sinks):
+    """Key 150 carries a value whose product with some upstream rows passes fp32: the rows that
+    see it are lost, as in the definition, and no other row is."""
+    n = 300
+    q, k, v = make(1, 2, 2, n, n, d, seed=5)
+    do = upstream(q)
+    want = ref.window_grad_ref(q, k, v, do, window, sinks, 1 / math.sqrt(d))
+    v[:, :, 150] = torch.finfo(v.dtype).max
+    dq, _, _ = grads_of(q, k, v, do, window, sinks)
+    away = ~ref.visible(n, n, window, sinks, "cuda")[:, 150]
+    g, lim = (x[:, :, away] for x in want["dq"])
+    assert ((dq[:, :, away].double() - g).abs() <= lim).all()
