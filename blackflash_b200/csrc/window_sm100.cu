@@ -113,10 +113,13 @@ extern "C" int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const b
     if ((rc = make_map_4d(&mk, K->data, f16, dk, tk, 128, 1)) != BF_OK) return rc;
     if ((rc = make_map_4d(&mv, V->data, f16, dk, tv, 128, 1)) != BF_OK) return rc;
     // Sinks in a step of 32 columns where they fit one: at N = 8192 with 4 sinks, d = 64, window
-    // 1024 it takes 235 -> 209 us, d = 128, window 128 130 -> 122. At d = 128 and window 1024 it
-    // takes 303 -> 314 (the larger kernel's full steps are scheduled worse), so there only for
-    // short windows.
-    const bool narrow = p.sinks > 0 && p.sinks <= 32 && (d == 64 || p.window <= 384);
+    // 1024 it takes 235 -> 209 us. At d = 128 the larger kernel's full steps are scheduled worse, so
+    // there only for short windows. us full / narrow at d = 128, 4 sinks (1 and 32 alike), by window:
+    //                           256          384          512          640          768
+    //   B=4 Hq=16 Hkv=4 N=8192  167 / 161    191 / 188    219 / 218    244 / 246    277 / 282
+    //   B=2 H=16 N=4096         58.9 / 55.0  66.6 / 63.8  71.9 / 70.7  77.6 / 77.2  83.2 / 83.5
+    //   B=4 Hq=8 Hkv=2 N=2048   27.5 / 25.5  31.3 / 29.9  35.2 / 34.0  38.9 / 38.1  40.7 / 41.1
+    const bool narrow = p.sinks > 0 && p.sinks <= 32 && (d == 64 || p.window <= 512);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return narrow ? launch_fwd<false, true>(d, f16, mq, mk, mv, p, st) : launch_fwd<false, false>(d, f16, mq, mk, mv, p, st);
 }

@@ -289,3 +289,11 @@ def test_window_backward_late_blocks(b, h, n, window, sinks):
     got = grads_of(q, k, v, do, window, sinks)
     check_grads(got, q, k, v, do, window, sinks)
     assert all(torch.equal(x, y) for x, y in zip(got, grads_of(q, k, v, do, window, sinks)))
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sinks", [1, 32, 33])
+@pytest.mark.parametrize("window", [512, 513])
+def test_window_sides_of_the_narrow_sink_step(t, sinks, window):
+    """At d = 128 the sinks have a step of 32 columns up to window 512."""
+    run_and_check(*make(1, 4, 2, 1100, 1100, 128, t, seed=sinks), window, sinks)
