@@ -4,9 +4,10 @@
 // A step reads every visible key and value once and computes 2 * rows products per element
 // read, rows = group * T (query heads of a KV head times new tokens): far below the
 // 250 operations a byte at which the tensor core would bound it, so the kernel is built
-// for bytes in flight. A block is four warps that share nothing but the last join: each
-// walks its own 16-byte cp.async pipeline over groups of keys, multiplies them with all 16
-// rows of the tile by m16n8k16, and keeps its own running maximum, sum and output. Keys
+// for bytes in flight. A block is four warps (eight where it takes few keys and has a
+// multiprocessor to itself) that share nothing but the last join: each walks its own 16-byte
+// cp.async pipeline over groups of keys, multiplies them with all 16 rows of the tile by
+// m16n8k16, and keeps its own running maximum, sum and output. Keys
 // past a sequence's length are filled with zeros in shared memory and never read from
 // memory, so what a cache holds there (infinities, NaN, addresses past its end) does not
 // matter. The visible keys of a row tile are [0, s0) and [lo, hi); they are numbered
@@ -568,10 +569,23 @@ int make_plan(int B, int Hq, int Hkv, int T, int P, int C, int d, int window, in
             p.splits = (int)n;
         }
     }
-    // Few keys: one block of eight warps a unit and no join, for as many steps a warp as the
-    // units leave multiprocessors idle. us in a graph, wide / split, by units and keys at d = 128:
-    // 8 units, 516 keys 7.2 / 5.7; 64 units, 384 6.0 / 6.9 and 516 7.7 / 7.5; 128 units, 1000 11.4 / 12.5
-    // (wide is one launch instead of two besides, 3 us of the host's).
+    // Few keys: one block of eight warps a unit and no join. That saves the parts' way through
+    // memory and a launch, which is 3.1 us of the host's where calls follow one another and nothing
+    // in a graph; but it leaves the other multiprocessors idle. us in a graph, split / wide, by
+    // steps a warp (256 keys at d = 64, 128 at d = 128):
+    //                        2           3           4           6            8
+    //   d=64,   1 unit    4.5 / 4.3   4.3 / 5.3   4.5 / 6.5   5.3 / 8.5    5.5 / 10.7
+    //          48 units   5.7 / 4.6   6.0 / 5.7   6.3 / 6.8   7.0 / 8.9    7.6 / 11.0
+    //          96 units   6.4 / 4.7   6.9 / 5.9   7.6 / 7.0   8.9 / 9.1   10.4 / 11.3
+    //         144 units   7.3 / 4.7   7.7 / 5.8   8.9 / 6.9  10.4 / 9.1   13.3 / 11.3
+    //   d=128,  1 unit    4.9 / 4.6   5.3 / 5.6   5.5 / 6.7   5.7 / 8.7    5.5 / 10.8
+    //          48 units   5.3 / 4.8   6.3 / 6.1   7.0 / 7.1   7.7 / 9.1    8.3 / 11.1
+    //          96 units   6.7 / 5.0   7.6 / 6.1   8.4 / 7.2   9.6 / 9.3   11.2 / 11.4
+    //         144 units   7.5 / 5.0  10.1 / 6.1   9.5 / 7.2  12.8 / 9.3   15.4 / 11.4
+    // From 48 units on wide is taken for units / 16 steps, up to which it is no slower in a graph
+    // either (3 % at most). Below that for three: the third step costs up to 1 us in a graph at d = 64
+    // (0.3 at d = 128) and spares calls outside of one their second launch (9.1 -> 5.9 us); a fourth
+    // would cost 2 us for the same.
     const long long keys = 2048 / d, steps = (vis + bfk::dec::kWideWarps * keys - 1) / (bfk::dec::kWideWarps * keys);
     p.wide = units <= kPlanSms && vis > bfk::dec::kWarps * keys && steps <= (units > 48 ? units / 16 : 3);
     if (p.wide) {
