@@ -48,14 +48,10 @@ EXPORTED = (
 _lock = threading.Lock()
 _lib = None
 
-# Element types (BF_DTYPE_*).
-DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
-
 
 class View(ctypes.Structure):
     """bf_view: address and the element strides of batch, head and token."""
     _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_longlong * 3)]
-
 
 
 _vp, _fp, _i, _ll, _f = ctypes.c_void_p, ctypes.POINTER(ctypes.c_float), ctypes.c_int, ctypes.c_longlong, ctypes.c_float

@@ -51,7 +51,8 @@ def window_attention_lse(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, wind
     the keys j <= p with j > p - window or j < sinks; window >= Nkv is causal attention.
     Returns (O [B, Hq, Nq, d], lse [B, Hq, Nq] fp32); a query that sees no key (p < 0) gets
     0 and -inf. K and V must be finite in every row, those of padding too: a masked key has
-    weight 0, but 0 times an infinity or NaN is NaN.
+    weight 0, but 0 times an infinity or NaN is NaN. A row that sees a score of NaN or +inf is
+    NaN.
     """
     _tensors(Q=Q, K=K, V=V)
     return _ext().window_lse(Q, K, V, min(window, _MAX), min(sinks, _MAX), scale, want_lse)
@@ -93,7 +94,8 @@ def window_decode(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor,
     (held to 0 .. C); new token t stands at position p = lengths[b] - T + t and sees the
     keys j <= p with j > p - window or j < sinks. Returns O [B, Hq, T, d], or (O, lse) with
     want_lse; a token that sees no key (p < 0) gets 0 and -inf. Cache rows at lengths[b]
-    and after are never read and may hold anything.
+    and after are never read and may hold anything; V's rows of the step's own tokens and of
+    its window must be finite, for the other tokens too.
     """
     _tensors(Q=Q, K_cache=K_cache, V_cache=V_cache, lengths=lengths)
     O, lse = _ext().window_decode(Q, K_cache, V_cache, lengths, min(window, _MAX), min(sinks, _MAX), scale, want_lse)

@@ -177,7 +177,8 @@ typedef struct {
  * keys j <= p with j > p - window or j < sinks. window >= Nkv is plain causal attention. A
  * query that sees no key (p < 0) gets O = 0 and lse = -inf. scale must be positive.
  * K and V must be finite in every row: a masked key has weight 0, but it takes part in the
- * matrix products of its 128-row tile, and 0 times an infinity or NaN is NaN.
+ * matrix products of its 128-row tile, and 0 times an infinity or NaN is NaN. Any finite
+ * value will do there. A row that sees a score of NaN or +inf is NaN, its lse too.
  */
 int blackflash_window_fwd(const bf_view* Q, const bf_view* K, const bf_view* V, void* O, float* lse, int B, int Hq,
                           int Hkv, int Nq, int Nkv, int d, int window, int sinks, float scale, int dtype, void* stream);
@@ -199,16 +200,18 @@ int blackflash_window_bwd(const bf_view* Q, const bf_view* K, const bf_view* V, 
 /*
  * Decoding steps: T >= 1 new tokens of each sequence against its cache. No counterpart in
  * the reference.
- *   Q: [B, Hq, T, d] contiguous; K, V: caches [B, Hkv, C, d] of any strides; lengths: [B]
- *   int32 on the device, the tokens of each cache in use, the T new ones among them (held
- *   to 0 .. C). O: [B, Hq, T, d] contiguous; lse: [B, Hq, T] fp32, optional.
+ *   Q: [B, Hq, T, d] contiguous; K, V: caches [B, Hkv, C, d], strided as every bf_view; lengths:
+ *   [B] int32 on the device, the tokens of each cache in use, the T new ones among them (held
+ *   to 0 .. C). O: [B, Hq, T, d] contiguous; lse: [B, Hq, T] fp32, optional. Q and O are 16-byte
+ *   aligned.
  * New token t of sequence b stands at position p = lengths[b] - T + t. In
  * blackflash_window_decode it sees the keys j <= p with j > p - window or j < sinks; in
  * blackflash_prefix_decode all P keys of the prefix Kp, Vp [Hkv, P, d] that the sequences
  * share (axis 0 of their views is not looked at; its one batch element serves all) and
  * the keys j <= p of its own cache. P or C may be 0 (then the matching views may be null).
  * A token that sees no key gets O = 0 and lse = -inf. Cache rows at lengths[b] and after are
- * never read.
+ * never read. V must be finite in the rows in use that a token does not see (those of later
+ * tokens of the step, and those that leave its window within it): they have weight 0 in its products.
  *   workspace: device memory of blackflash_decode_workspace_bytes(...) bytes (P = 0 for
  *   blackflash_window_decode; window = INT_MAX and sinks = 0 for blackflash_prefix_decode),
  *   32-byte aligned, overwritten; null where that is 0. It returns -1 for bad sizes. Calls
@@ -231,7 +234,8 @@ int blackflash_prefix_decode(const void* Q, const bf_view* Kp, const bf_view* Vp
  * other way, which is the gradient's map.
  *   positions: [N], or [B, N] with positions_per_batch != 0; int32, or int64 with
  *   positions_64 != 0. freqs: [rotary_dim / 2] fp64. Both on the device.
- *   d even and at most 1024; addresses whole pairs, strides even and >= 0 (0 broadcasts).
+ *   d even and at most 1024; addresses, the outputs' too, at whole pairs (twice the element's size),
+ *   strides even and >= 0 (0 broadcasts). 16-byte addresses, strides and pieces of a row are faster.
  */
 int blackflash_rotary(const bf_view* Q, const bf_view* K, void* Q_out, void* K_out, const void* positions,
                       int positions_64, int positions_per_batch, const double* freqs, int B, int Hq, int Hk, int N, int d,
