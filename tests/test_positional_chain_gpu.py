@@ -290,6 +290,34 @@ def test_captured_backward_through_other_operations():
     assert out.returncode == 0 and out.stdout.split("\n")[:-1] == lines, out.stdout + out.stderr[-2000:]
 
 
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_checkpointed_step_and_no_grad_modes(reentrant):
+    """Recomputed in the backward, the step has the same gradients; without gradients the same output."""
+    from torch.utils.checkpoint import checkpoint
+
+    from blackflash_b200 import rotary_frequencies, rotary_with_grad, window_attention, window_attention_with_grad
+    freqs, _ = rotary_frequencies(64)
+    pos = torch.arange(150, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(2, 150, 6, 64, generator=gen, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    do = torch.randn(2, 4, 150, 64, generator=gen, device="cuda").to(torch.bfloat16)
+
+    def layer(a):
+        q, k = rotary_with_grad(a[:, :, :4].transpose(1, 2), a[:, :, 4:].transpose(1, 2), pos, freqs)
+        return window_attention_with_grad(q, k, k, 40, 2)
+    o = layer(x)
+    want, = torch.autograd.grad(o, x, do)
+    layer_o = checkpoint(layer, x, use_reentrant=reentrant)
+    layer_o.backward(do)
+    assert torch.equal(layer_o, o) and torch.equal(x.grad, want)
+    with torch.no_grad():
+        assert torch.equal(layer(x), o)
+    with torch.inference_mode():
+        assert torch.equal(layer(x), o)
+        q = x[:, :, :4].transpose(1, 2)
+        assert torch.equal(window_attention(q, q, q, 40), window_attention_with_grad(q, q, q, 40))
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_other_device_than_the_current():
     import blackflash_b200 as bf

@@ -174,3 +174,44 @@ def test_backward_beside_partly_masked_keys_of_the_largest_size(d, window, sinks
     away = ~ref.visible(n, n, window, sinks, "cuda")[:, 150]
     g, lim = (x[:, :, away] for x in want["dq"])
     assert ((dq[:, :, away].double() - g).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,hkv,cap,window", [(16, 1, 300, 400), (16, 2, 3000, 2900), (16, 16, 60, 50), (16, 1, 12000, 11000)])
+def test_a_cache_key_of_nan_or_infinity_reaches_the_tokens_that_see_it(t, d, b, hkv, cap, window):
+    """One split and several, four warps a block and eight; three tokens, the last of which alone
+    see the key. It may hold the largest value where they do not."""
+    from blackflash_b200 import window_decode
+    tokens, base = 3, cap - 17
+    gen = torch.Generator(device="cuda").manual_seed(cap)
+
+    def rnd(*s):
+        return torch.randn(s, generator=gen, device="cuda").to(t)
+    q, k, v = rnd(b, 2 * hkv, tokens, d), rnd(b, hkv, cap, d), rnd(b, hkv, cap, d)
+    n = torch.full((b,), cap, dtype=torch.int32, device="cuda")
+    n[::2] = cap // 2
+    want, want_lse = window_decode(q, k, v, n, window, want_lse=True)
+    for value in (math.nan, math.inf):
+        bad = k.clone()
+        rows = torch.zeros(b, 2 * hkv, tokens, dtype=torch.bool, device="cuda")
+        for i in range(b):
+            key = (base + i) if i % 2 else cap // 2 - 1 - i % 3
+            bad[i, -1, key, 7] = value
+            pos = int(n[i]) - tokens + torch.arange(tokens, device="cuda")
+            seen = (key <= pos) & (key > pos - window)
+            # inf times a negative number is -inf, a weight of 0: looked at in the other test alone.
+            rows[i, -2:] = seen
+            if value == math.inf:
+                q[i, -2:, :, 7] = q[i, -2:, :, 7].abs() + 0.01
+        if value == math.inf:
+            want, want_lse = window_decode(q, k, v, n, window, want_lse=True)
+        got, lse = window_decode(q, bad, v, n, window, want_lse=True)
+        same_outside(got, want, rows)
+        same_outside(lse, want_lse, rows)
+    # The newest token's key and value at their largest: the tokens before it do not see them.
+    k2, v2 = k.clone(), v.clone()
+    for i in range(b):
+        k2[i, :, int(n[i]) - 1], v2[i, :, int(n[i]) - 1] = (torch.finfo(t).max * s for s in (-1, 1))
+    got = window_decode(q, k2, v2, n, window)
+    assert torch.equal(got[:, :, :-1], want[:, :, :-1])
