@@ -403,9 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!measure) {
                     // dP of a masked pair may pass fp32, of large finite numbers, and 0 times it is
                     // NaN: a word of dS that has one is looked for in masked steps, and only then are
-                    // the masked columns cleared. Looking takes 1.5 % of the backward at B=2 H=16
-                    // N=4096 d=64 window 1024 (182 -> 185 us), 3 % at window 256; clearing them in
-                    // each masked step 7 % and 15 %.
+                    // the masked columns cleared. Looking takes 2.5 % of the backward at B=2 H=16
+                    // N=4096 d=64 window 1024 (183 -> 187 us), 3.6 % at N=8192 window 256 (205 -> 213);
+                    // clearing them in each masked step 7 and 16 %.
                     if (edge) {
                         uint32_t t0 = 0u, t1 = 0u;
 #pragma unroll
